@@ -184,7 +184,7 @@ def _hipcc(args: list[str], what: str):
 def build_host(force: bool = False, jobs: int = 6):
     """Compile the Matrix<ROCMfloat> mirror and the reference's ROCm programs.
     Returns the list of binaries, or [] when the reference tree is absent."""
-    if not REFERENCE_ROOT.exists():
+    if not (REFERENCE_ROOT / "cpp").is_dir():   # not mounted, or an empty mount point
         return [*(sorted(REF_BIN.glob("*")) if REF_BIN.exists() else []), *(sorted(BIN.glob("*")) if BIN.exists() else [])]
     build()
     ov = make_overlay()

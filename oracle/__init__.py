@@ -86,7 +86,7 @@ def build(force: bool = False) -> Path:
 
 def build_ref(force: bool = False):
     """Compile the reference CPU path (oracle/_ref); None if the tree is absent."""
-    if not REFERENCE_ROOT.exists():
+    if not (REFERENCE_ROOT / "cpp").is_dir():   # not mounted, or an empty mount point
         return REF_LIB if REF_LIB.exists() else None
     r = subprocess.run(["make", "-C", str(HERE), "-s", f"REF={REFERENCE_ROOT}"] + (["-B"] if force else []),
                        capture_output=True, text=True)
