@@ -430,6 +430,88 @@ int jzhip_softmax_xent(float* loss_out, float* dlogits, const float* logits,
 int jzhip_softmax_xent_dense(float* loss_out, float* dlogits, const float* logits, const float* target,
                              int K, int N, int ld, float inv_nb);
 
+/* ── losses on the logits of a language model ────────────────────────── */
+
+/* No reference counterpart: LogisticLayer (ml/layer.hpp:232-284) is the reference's only
+ * loss over classes.  These take the same K x N logits (one token per column, leading
+ * dimension ld) and serve the training that follows it: scoring tokens, learning from
+ * rewards, from preferences and from a teacher.  Common to all of them:
+ *   - p = softmax of a column.  A label outside [0, K), a weight of 0, and a column that
+ *     holds nothing but -inf make a token that is not scored: it adds to no sum, its
+ *     outputs and its gradient are 0, and its logits, log-probabilities and advantage
+ *     (NaN and infinities included) are not looked at.  Entries of -inf, or of the type's
+ *     lowest value beside larger ones, have probability 0 and gradient 0.  A NaN in a column
+ *     that is scored reaches that column's outputs.
+ *   - dlogits (K x N, leading dimension ldd) may be NULL where only values are wanted, and
+ *     may be logits itself with ldd == ld; otherwise outputs overlap no input.  ldd - K
+ *     entries behind each column are left as they are.
+ *   - sums over a column are kept in fp32 and every per-token quantity derived from them
+ *     (log-probability, ratio, divergence) and every sum over tokens in 64 bits, all in a
+ *     fixed order: equal inputs give equal bits.
+ *   - scratch: caller-provided, 16-byte aligned, jzhip_token_scratch_floats(N, top) =
+ *     (8 + top) * N + 2^20 floats (top: 0 but for jzhip_distill_topk; for
+ *     jzhip_preference_loss N is the number of tokens).  Nothing in it outlives a call, and no
+ *     library workspace is used: calls with different scratch, outputs and inputs may run on
+ *     different streams or in different recorded graphs at the same time. */
+size_t jzhip_token_scratch_floats(int N, int top);
+/* logp[n] = log p(label_n), entropy[n] = -sum_i p_i log p_i (nats) and, for the gradient
+ * call below, stats: the N column maxima followed by the N sums of exp(x - max) (both 0 for
+ * a token that is not scored).  Each output may be NULL, not all three. */
+int jzhip_token_logprobs(float* logp, float* entropy, float* stats, float* scratch,
+                         const float* logits, const int32_t* labels, int K, int N, int ld);
+/* dlogits(i, n) = dlogp[n] * ([i == label_n] - p_i): the gradient of any function of those
+ * log-probabilities from the function's own gradient dlogp.  Columns whose dlogp is 0 become
+ * 0 without a look at their logits. */
+int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const float* logits,
+                             const int32_t* labels, const float* stats, int K, int N, int ld,
+                             int ldd);
+/* The clipped policy-gradient loss of sampled tokens (the labels), in one pass over the
+ * logits.  With r = p(label)/exp(old_logp), A = advantage, u = ref_logp - log p(label):
+ *   L = sum_n w_n * ( -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *                     + kl_coef * (e^u - u - 1) - entropy_coef * H_n )
+ * sums (4 floats): L, sum w (e^u - u - 1), sum w [the clamped branch is the smaller], and
+ * sum w H (0 when entropy_coef is 0: H is then not formed).  weight carries every mask and
+ * mean (1/tokens, 1/length of the answer); NULL: all 1.  ref_logp may be NULL when kl_coef
+ * is 0.  logp (N, may be NULL): log p(label).  Coefficients are not negative, clip_low <= 1. */
+int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* scratch,
+                      const float* logits, const int32_t* labels, const float* old_logp,
+                      const float* ref_logp, const float* advantage, const float* weight, int K,
+                      int N, int ld, int ldd, float clip_low, float clip_high, float kl_coef,
+                      float entropy_coef);
+/* The paired log-ratio loss of preference data.  seq_begin: 2*pairs + 1 column numbers on the
+ * HOST (read during the call; a recorded graph replays them), the first 0, never decreasing:
+ * sequence s is columns [seq_begin[s], seq_begin[s+1]), 2p the chosen and 2p + 1 the rejected
+ * answer of pair p; a sequence may be empty.  The columns behind the last sequence are not
+ * touched.  ref_logp: log-probabilities of the same tokens under the reference model
+ * (jzhip_token_logprobs), NULL for none.
+ *   R_s = beta * sum (log p(label) - ref_logp) over its scored tokens, divided by their number
+ *   when average != 0 (0 if there is none);  h_p = R_2p - R_2p+1
+ *   kind 0: l = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)   (smoothing < 0.5)
+ *   kind 1: l = max(0, 1 - h)         kind 2: l = ((h - 1/2) / beta)^2    (smoothing 0)
+ * loss_out[0] = scale * sum_p l(h_p), rewards (2*pairs) = R, logp and stats as
+ * jzhip_token_logprobs writes them (both needed), dlogits the gradient of loss_out.  A pair's
+ * gradient depends on all of its tokens, so the logits are read twice.  At most 2^18 pairs. */
+int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* stats,
+                          float* dlogits, float* scratch, const float* logits,
+                          const int32_t* labels, const float* ref_logp, const int* seq_begin,
+                          int pairs, int K, int ld, int ldd, int kind, float beta,
+                          float smoothing, int average, float scale);
+/* Distillation from the `top` largest logits of a teacher (at most 512): teacher and ids are
+ * top x N with leading dimension ldt.  An id outside [0, K) is no entry (fewer than `top`
+ * known), and of equal ids in a column only the first counts.  With T = temperature,
+ * q_j = exp(teacher_j / T - lse), the student's p = softmax(x / T):
+ *   teacher_lse == NULL: lse over the column's entries,
+ *       l = T^2 * sum_j q_j log(q_j / p(id_j))
+ *   teacher_lse (N): log sum exp(teacher / T) over the teacher's whole vocabulary; what the
+ *       entries leave, max(0, 1 - sum q_j), is one more class against the p of everything else.
+ * loss_out[0] = sum_n w_n l_n (weight NULL: all 1), token_loss (N, may be NULL) = l_n, dlogits
+ * the gradient of loss_out.  A column without entries (or, with teacher_lse NULL, of entries
+ * of -inf only) is not scored.  temperature in [1e-3, 1e3]. */
+int jzhip_distill_topk(float* loss_out, float* token_loss, float* dlogits, float* scratch,
+                       const float* logits, const float* teacher, const int32_t* ids,
+                       const float* teacher_lse, const float* weight, int K, int top, int N,
+                       int ld, int ldd, int ldt, float temperature);
+
 /* Multi-head self-attention core over the layouts TransformerLayer keeps
  * (ml/layer.hpp:2843-2848): Q, K, V, H are (d_k, S*B) column-major with head hh
  * in rows [hh*d_h, (hh+1)*d_h) and sequence b in columns [b*S, (b+1)*S); A is

@@ -120,6 +120,12 @@ SIGNATURES: dict[str, tuple] = {
     "jzhip_attn_softmax_bwd": (I, [P, P, P, I, I, F, I]),
     "jzhip_softmax_xent": (I, [P, P, P, P, I, I, I]),
     "jzhip_softmax_xent_dense": (I, [P, P, P, P, I, I, I, F]),
+    "jzhip_token_scratch_floats": (Z, [I, I]),
+    "jzhip_token_logprobs": (I, [P, P, P, P, P, P, I, I, I]),
+    "jzhip_token_logprobs_bwd": (I, [P, P, P, P, P, I, I, I, I]),
+    "jzhip_policy_loss": (I, [P] * 10 + [I] * 4 + [F] * 4),
+    "jzhip_preference_loss": (I, [P] * 9 + [C.POINTER(C.c_int)] + [I] * 5 + [F, F, I, F]),
+    "jzhip_distill_topk": (I, [P] * 9 + [I] * 6 + [F]),
     "jzhip_attention_fwd_ld": (I, [P, I, P, P, P, P, I, I, I, I, I, I]),
     "jzhip_attention_bwd_ld": (I, [P, P, P, I, P, P, I, P, P, P, I, P, I, I, I, I, I]),
     "jzhip_attention_flash_supported": (I, [I, I, I, I]),

@@ -1,0 +1,202 @@
+// Log-probabilities of one label per token, their gradient, and the paired
+// log-ratio (preference) loss built on the two.
+#include "token_loss.hpp"
+
+namespace jz {
+namespace {
+
+struct NoShared {};
+
+template <bool ENTROPY>
+struct LogprobHead {
+    static constexpr bool kEntropy = ENTROPY, kRest = false;
+    using Shared = NoShared;
+    ExpScale scale;
+    const int32_t* labels;
+    float *logp, *entropy, *stats;   // each may be null
+    int N;
+
+    __device__ bool live(size_t col, int K) const { return label_scored(labels[col], K); }
+    template <class T>
+    __device__ bool prologue(const T&, Shared&, size_t, int) const { return true; }
+    __device__ void write(size_t col, float lp, float h, float m, float s) const {
+        if (logp) logp[col] = lp;
+        if (ENTROPY) entropy[col] = h;
+        if (stats) {
+            stats[col] = m;
+            stats[static_cast<size_t>(N) + col] = s;
+        }
+    }
+    __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f); }
+    template <class T>
+    __device__ Coef finish(const T& team, Shared&, size_t col, const ColumnSums& c, const float* x) const {
+        if (team.rank == 0)
+            write(col, static_cast<float>(log_prob(x[labels[col]], c)),
+                  ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f, c.m, c.s);
+        return Coef{0.f, 0.f};
+    }
+    template <class T>
+    __device__ void correct(const T&, Shared&, size_t, const ColumnSums&, const Coef&, float*) const {}
+};
+
+// d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
+// is left, every element is read and written once.
+constexpr int kBwdBlock = 256;
+__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const float* g, const float* x,
+                                                                const int32_t* labels, const float* stats, int K,
+                                                                int N, size_t ld, size_t ldd, ExpScale scale) {
+    const size_t col = blockIdx.x;
+    const float* p = x + col * ld;
+    float* out = d + col * ldd;
+    const int label = labels[col];
+    const float up = g[col], m = stats[col], s = stats[static_cast<size_t>(N) + col];
+    const bool live = label_scored(label, K) && s != 0.f && up != 0.f;
+    const float a = live ? static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)) : 0.f;
+    for (int i = threadIdx.x; i < K; i += kBwdBlock) {
+        float v = 0.f;
+        if (live) {
+            v = exp_shifted(p[i] - m, scale) * a;
+            if (i == label) v += up;
+        }
+        out[i] = v;
+    }
+}
+
+int logprobs(float* logp, float* entropy, float* stats, const float* x, const int32_t* labels, int K, int N,
+             size_t ld) {
+    if (entropy)
+        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, nullptr, x, K,
+                                   N, ld, ld);
+    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, nullptr, x, K, N,
+                               ld, ld);
+}
+
+int logprobs_bwd(float* d, const float* g, const float* x, const int32_t* labels, const float* stats, int K, int N,
+                 size_t ld, size_t ldd) {
+    logprob_bwd_kernel<<<static_cast<unsigned>(N), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N, ld, ldd,
+                                                                             exp_scale(1.0));
+    return launch_rc();
+}
+
+// ── paired log ratios ────────────────────────────────────────────────────
+// R_s = beta * sum over the scored tokens of sequence s of (logp - ref) [/ their number],
+// h = R_chosen - R_rejected.  The slope dl/dh scales both sequences' gradients, so every
+// log-probability of a pair is needed before the first gradient of it can be written:
+// logprobs over the columns, this kernel over the pairs, logprobs_bwd over the columns.
+enum PreferenceKind { kSigmoid = 0, kHinge = 1, kSquared = 2 };
+
+constexpr int kPairsPerLaunch = 64;
+struct PairBegins {
+    int at[2 * kPairsPerLaunch + 1];
+};
+constexpr int kPairBlock = 256;
+__global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(
+    float* g, float* rewards, double* losses, const float* x, const int32_t* labels, const float* stats,
+    const float* ref, PairBegins begins, int K, int N, size_t ld, int kind, float beta, float smoothing, int average,
+    float scale) {
+    __shared__ double red[kPairBlock / kWave];
+    const Team<kPairBlock> team{static_cast<int>(threadIdx.x), red};
+    const int pair = blockIdx.x;
+    double reward[2], share[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int lo = begins.at[2 * pair + k], hi = begins.at[2 * pair + k + 1];
+        double gain = 0.0, count = 0.0;
+        for (int n = lo + team.rank; n < hi; n += kPairBlock) {
+            const int label = labels[n];
+            const float s = stats[static_cast<size_t>(N) + n];
+            if (!label_scored(label, K) || s == 0.f) continue;
+            const ColumnSums c{stats[n], s, 0.f, 0.f};
+            gain += log_prob(x[static_cast<size_t>(n) * ld + label], c) - (ref ? static_cast<double>(ref[n]) : 0.0);
+            count += 1.0;
+        }
+        gain = team.sum(gain);
+        count = team.sum(count);
+        share[k] = average ? (count > 0.0 ? 1.0 / count : 0.0) : 1.0;
+        reward[k] = static_cast<double>(beta) * gain * share[k];
+    }
+    const double h = reward[0] - reward[1];
+    double loss, slope;   // of h; the comparisons are written so that a NaN stays one
+    if (kind == kSigmoid) {
+        const double z = exp(-fabs(h)), tail = log1p(z);
+        const double down = (h >= 0.0 ? z : 1.0) / (1.0 + z), up = (h >= 0.0 ? 1.0 : z) / (1.0 + z);   // sigma(-h), sigma(h)
+        const double sm = static_cast<double>(smoothing);
+        loss = (1.0 - sm) * (tail + (h >= 0.0 ? 0.0 : -h)) + sm * (tail + (h >= 0.0 ? h : 0.0));
+        slope = -(1.0 - sm) * down + sm * up;
+    } else if (kind == kHinge) {
+        loss = h >= 1.0 ? 0.0 : 1.0 - h;
+        slope = h >= 1.0 ? 0.0 : (h < 1.0 ? -1.0 : h);
+    } else {
+        const double off = (h - 0.5) / static_cast<double>(beta);
+        loss = off * off;
+        slope = 2.0 * off / static_cast<double>(beta);
+    }
+    if (team.rank == 0) {
+        rewards[2 * pair] = static_cast<float>(reward[0]);
+        rewards[2 * pair + 1] = static_cast<float>(reward[1]);
+        losses[pair] = loss;
+    }
+    if (!g) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const double v = (k ? -slope : slope) * share[k] * static_cast<double>(beta) * static_cast<double>(scale);
+        for (int n = begins.at[2 * pair + k] + team.rank; n < begins.at[2 * pair + k + 1]; n += kPairBlock)
+            g[n] = static_cast<float>(v);
+    }
+}
+
+}  // namespace
+}  // namespace jz
+
+using namespace jz;
+
+JZ_API size_t jzhip_token_scratch_floats(int N, int top) {
+    if (N <= 0 || top < 0) return 0;
+    return (static_cast<size_t>(8) + static_cast<size_t>(top)) * static_cast<size_t>(N) + (size_t(1) << 20);
+}
+
+JZ_API int jzhip_token_logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* logits,
+                                const int32_t* labels, int K, int N, int ld) {
+    if (!token_args_ok(logits, nullptr, scratch, K, N, ld, ld) || !labels || !scratch || (!logp && !entropy && !stats))
+        return -1;
+    return logprobs(logp, entropy, stats, logits, labels, K, N, static_cast<size_t>(ld));
+}
+
+JZ_API int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const float* logits, const int32_t* labels,
+                                    const float* stats, int K, int N, int ld, int ldd) {
+    if (!token_args_ok(logits, dlogits, nullptr, K, N, ld, ldd) || !dlogits || !dlogp || !labels || !stats) return -1;
+    return logprobs_bwd(dlogits, dlogp, logits, labels, stats, K, N, static_cast<size_t>(ld),
+                        static_cast<size_t>(ldd));
+}
+
+JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* stats, float* dlogits,
+                                 float* scratch, const float* logits, const int32_t* labels, const float* ref_logp,
+                                 const int* seq_begin, int pairs, int K, int ld, int ldd, int kind, float beta,
+                                 float smoothing, int average, float scale) {
+    if (!loss_out || !rewards || !logp || !stats || !scratch || !labels || !seq_begin || pairs <= 0) return -1;
+    if (pairs > (1 << 18)) return -1;   // the pairs' losses fill half of the fixed part of the scratch
+    if (kind < kSigmoid || kind > kSquared || !(beta > 0.f) || !(smoothing >= 0.f && smoothing < 0.5f)) return -1;
+    if (kind != kSigmoid && smoothing != 0.f) return -1;
+    if (seq_begin[0] != 0) return -1;
+    for (int i = 0; i < 2 * pairs; ++i)
+        if (seq_begin[i + 1] < seq_begin[i]) return -1;
+    const int N = seq_begin[2 * pairs];
+    if (!token_args_ok(logits, dlogits, scratch, K, N, ld, ldd)) return -1;
+    double* losses = reinterpret_cast<double*>(scratch);
+    float* g = scratch + (size_t(1) << 20);
+    const size_t ldx = static_cast<size_t>(ld);
+    int rc = logprobs(logp, nullptr, stats, logits, labels, K, N, ldx);
+    for (int at = 0; rc == 0 && at < pairs; at += kPairsPerLaunch) {
+        const int n = pairs - at < kPairsPerLaunch ? pairs - at : kPairsPerLaunch;
+        PairBegins begins = {};
+        for (int i = 0; i <= 2 * n; ++i) begins.at[i] = seq_begin[2 * at + i];
+        preference_pair_kernel<<<n, kPairBlock, 0, stream()>>>(dlogits ? g : nullptr, rewards + 2 * at, losses + at,
+                                                               logits, labels, stats, ref_logp, begins, K, N, ldx,
+                                                               kind, beta, smoothing, average, scale);
+        rc = launch_rc();
+    }
+    if (rc == 0 && dlogits) rc = logprobs_bwd(dlogits, g, logits, labels, stats, K, N, ldx, static_cast<size_t>(ldd));
+    if (rc) return rc;
+    token_fold_kernel<double><<<1, kFoldBlock, 0, stream()>>>(loss_out, losses, pairs, 0, static_cast<double>(scale));
+    return launch_rc();
+}
