@@ -5,20 +5,19 @@
 namespace jz {
 namespace {
 
-struct NoShared {};
-
 template <bool ENTROPY>
 struct LogprobHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false;
-    using Shared = NoShared;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeamwork = false, kWrites = false;
     ExpScale scale;
     const int32_t* labels;
     float *logp, *entropy, *stats;   // each may be null
     int N;
 
+    __host__ __device__ size_t team_bytes(int) const { return 0; }
     __device__ bool live(size_t col, int K) const { return label_scored(labels[col], K); }
+    __device__ int label(size_t col) const { return labels[col]; }
     template <class T>
-    __device__ bool prologue(const T&, Shared&, size_t, int) const { return true; }
+    __device__ bool prologue(const T&, char*, size_t, int) const { return true; }
     __device__ void write(size_t col, float lp, float h, float m, float s) const {
         if (logp) logp[col] = lp;
         if (ENTROPY) entropy[col] = h;
@@ -29,53 +28,95 @@ struct LogprobHead {
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f); }
     template <class T>
-    __device__ Coef finish(const T& team, Shared&, size_t col, const ColumnSums& c, const float* x) const {
-        if (team.rank == 0)
-            write(col, static_cast<float>(log_prob(x[labels[col]], c)),
-                  ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f, c.m, c.s);
-        return Coef{0.f, 0.f};
+    __device__ Grad finish(const T& team, char*, size_t col, const ColumnSums& c, const float* x) const {
+        if (team.leads()) {
+            const float lp = static_cast<float>(log_prob(x[labels[col]], c));
+            const float h = ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f;
+            if (team.rank == 0) write(col, lp, h, c.m, static_cast<float>(c.s));
+        }
+        return Grad{};
     }
     template <class T>
-    __device__ void correct(const T&, Shared&, size_t, const ColumnSums&, const Coef&, float*) const {}
+    __device__ void correct(const T&, char*, size_t, float, const Grad&, float*, int) const {}
 };
 
 // d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
-// is left, every element is read and written once.
-constexpr int kBwdBlock = 256;
+// is left, every element is read and written once.  A team of G threads takes 16*G
+// logits of a column.
+constexpr int kBwdBlock = 256, kBwdQuads = 4;
+template <int G>
 __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const float* g, const float* x,
                                                                 const int32_t* labels, const float* stats, int K,
-                                                                int N, size_t ld, size_t ldd, ExpScale scale) {
-    const size_t col = blockIdx.x;
-    const float* p = x + col * ld;
-    float* out = d + col * ldd;
+                                                                int N, int chunks, size_t ld, size_t ldd,
+                                                                ExpScale scale) {
+    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
+    const Team<G> team{static_cast<int>(threadIdx.x % G), nullptr};
+    const size_t piece = static_cast<size_t>(blockIdx.x) * kTeams + threadIdx.x / G;
+    const size_t col = kTeams > 1 ? piece : piece / chunks;
+    if (col >= static_cast<size_t>(N)) return;
+    const int begin = kTeams > 1 ? 0 : static_cast<int>(piece % chunks) * kSpan;
+    const int len = K - begin < kSpan ? K - begin : kSpan;
+    const int quads = len / 4, odd = len % 4;
+    const float* p = x + col * ld + begin;
+    float* out = d + col * ldd + begin;
     const int label = labels[col];
     const float up = g[col], m = stats[col], s = stats[static_cast<size_t>(N) + col];
     const bool live = label_scored(label, K) && s != 0.f && up != 0.f;
-    const float a = live ? static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)) : 0.f;
-    for (int i = threadIdx.x; i < K; i += kBwdBlock) {
-        float v = 0.f;
-        if (live) {
-            v = exp_shifted(p[i] - m, scale) * a;
-            if (i == label) v += up;
-        }
-        out[i] = v;
+    if (!live) {
+        for (int q = team.rank; q < quads; q += G) *reinterpret_cast<Quad*>(out + 4 * q) = Quad(0.f);
+        if (team.rank < odd) out[4 * quads + team.rank] = 0.f;
+        return;
     }
+    Quad v[kBwdQuads];
+#pragma unroll
+    for (int k = 0; k < kBwdQuads; ++k) {
+        const int q = team.rank + k * G;
+        if (q < quads) v[k] = *reinterpret_cast<const Quad*>(p + 4 * q);
+    }
+    const float last = team.rank < odd ? p[4 * quads + team.rank] : 0.f;
+    const bool mine = label >= begin && label < begin + len;
+    Grad f{static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)), 0.f, up, 0.f};
+    if (mine) {
+        f.x = p[label - begin];
+        if constexpr (kTeams == 1) __syncthreads();   // the gradient may replace the logits
+        else team.sync();
+    }
+    auto value = [&](float y) { return exp_shifted(y - m, scale) * f.a; };
+#pragma unroll
+    for (int k = 0; k < kBwdQuads; ++k) {
+        const int q = team.rank + k * G;
+        if (q < quads) *reinterpret_cast<Quad*>(out + 4 * q) = Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)};
+    }
+    if (team.rank < odd) out[4 * quads + team.rank] = value(last);
+    if (mine) correct_label<false>(team, label - begin, quads, m, f, scale, out);
 }
 
-int logprobs(float* logp, float* entropy, float* stats, const float* x, const int32_t* labels, int K, int N,
-             size_t ld) {
+int logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* x, const int32_t* labels, int K,
+             int N, size_t ld) {
     if (entropy)
-        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, nullptr, x, K,
-                                   N, ld, ld);
-    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, nullptr, x, K, N,
-                               ld, ld);
+        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, scratch,
+                                   nullptr, x, K, N, ld, ld);
+    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, scratch, nullptr,
+                               x, K, N, ld, ld);
+}
+
+template <int G>
+int launch_bwd(float* d, const float* g, const float* x, const int32_t* labels, const float* stats, int K, int N,
+               size_t ld, size_t ldd) {
+    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
+    const int chunks = kTeams > 1 ? 1 : (K + kSpan - 1) / kSpan;
+    const size_t blocks = (static_cast<size_t>(N) * chunks + kTeams - 1) / kTeams;
+    logprob_bwd_kernel<G><<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N,
+                                                                                     chunks, ld, ldd, exp_scale(1.0));
+    return launch_rc();
 }
 
 int logprobs_bwd(float* d, const float* g, const float* x, const int32_t* labels, const float* stats, int K, int N,
                  size_t ld, size_t ldd) {
-    logprob_bwd_kernel<<<static_cast<unsigned>(N), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N, ld, ldd,
-                                                                             exp_scale(1.0));
-    return launch_rc();
+    if (K <= 64) return launch_bwd<4>(d, g, x, labels, stats, K, N, ld, ldd);
+    if (K <= 256) return launch_bwd<16>(d, g, x, labels, stats, K, N, ld, ldd);
+    if (K <= 1024) return launch_bwd<64>(d, g, x, labels, stats, K, N, ld, ldd);
+    return launch_bwd<256>(d, g, x, labels, stats, K, N, ld, ldd);
 }
 
 // ── paired log ratios ────────────────────────────────────────────────────
@@ -106,7 +147,7 @@ __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(
             const int label = labels[n];
             const float s = stats[static_cast<size_t>(N) + n];
             if (!label_scored(label, K) || s == 0.f) continue;
-            const ColumnSums c{stats[n], s, 0.f, 0.f};
+            const ColumnSums c{stats[n], static_cast<double>(s), 0.0, 0.0};
             gain += log_prob(x[static_cast<size_t>(n) * ld + label], c) - (ref ? static_cast<double>(ref[n]) : 0.0);
             count += 1.0;
         }
@@ -152,14 +193,14 @@ using namespace jz;
 
 JZ_API size_t jzhip_token_scratch_floats(int N, int top) {
     if (N <= 0 || top < 0) return 0;
-    return (static_cast<size_t>(8) + static_cast<size_t>(top)) * static_cast<size_t>(N) + (size_t(1) << 20);
+    return (static_cast<size_t>(8) + static_cast<size_t>(top)) * static_cast<size_t>(N) + kScratchFixed;
 }
 
 JZ_API int jzhip_token_logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* logits,
                                 const int32_t* labels, int K, int N, int ld) {
     if (!token_args_ok(logits, nullptr, scratch, K, N, ld, ld) || !labels || !scratch || (!logp && !entropy && !stats))
         return -1;
-    return logprobs(logp, entropy, stats, logits, labels, K, N, static_cast<size_t>(ld));
+    return logprobs(logp, entropy, stats, scratch, logits, labels, K, N, static_cast<size_t>(ld));
 }
 
 JZ_API int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const float* logits, const int32_t* labels,
@@ -183,9 +224,9 @@ JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, f
     const int N = seq_begin[2 * pairs];
     if (!token_args_ok(logits, dlogits, scratch, K, N, ld, ldd)) return -1;
     double* losses = reinterpret_cast<double*>(scratch);
-    float* g = scratch + (size_t(1) << 20);
+    float* g = scratch + kScratchFixed;
     const size_t ldx = static_cast<size_t>(ld);
-    int rc = logprobs(logp, nullptr, stats, logits, labels, K, N, ldx);
+    int rc = logprobs(logp, nullptr, stats, scratch, logits, labels, K, N, ldx);
     for (int at = 0; rc == 0 && at < pairs; at += kPairsPerLaunch) {
         const int n = pairs - at < kPairsPerLaunch ? pairs - at : kPairsPerLaunch;
         PairBegins begins = {};

@@ -12,16 +12,9 @@
 namespace jz {
 namespace {
 
-struct PolicyShared {
-    float g;   // dL/dlogp
-    float x;   // the label's logit
-    Coef f;
-};
-
 template <bool ENTROPY>
 struct PolicyHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false;
-    using Shared = PolicyShared;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeamwork = false, kWrites = true;
     ExpScale scale;
     const int32_t* labels;
     const float *old_logp, *ref_logp, *advantage, *weight;   // ref_logp, weight may be null
@@ -29,11 +22,13 @@ struct PolicyHead {
     float clip_low, clip_high, kl_coef, entropy_coef;
     int N;
 
+    __host__ __device__ size_t team_bytes(int) const { return 0; }
     __device__ bool live(size_t col, int K) const {
         return label_scored(labels[col], K) && !(weight && weight[col] == 0.f);
     }
+    __device__ int label(size_t col) const { return labels[col]; }
     template <class T>
-    __device__ bool prologue(const T&, Shared&, size_t, int) const { return true; }
+    __device__ bool prologue(const T&, char*, size_t, int) const { return true; }
     __device__ void write(size_t col, float lp, float loss, float kl, float cut, float h) const {
         const size_t n = static_cast<size_t>(N);
         if (logp) logp[col] = lp;
@@ -44,51 +39,48 @@ struct PolicyHead {
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f, 0.f); }
     template <class T>
-    __device__ Coef finish(const T& team, Shared& sh, size_t col, const ColumnSums& c, const float* x) const {
-        if (team.rank == 0) {
-            const double w = weight ? static_cast<double>(weight[col]) : 1.0;
-            const double adv = static_cast<double>(advantage[col]);
-            const float xl = x[labels[col]];
-            const double lp = log_prob(xl, c);
-            const double ratio = exp(lp - static_cast<double>(old_logp[col]));
-            const double low = 1.0 - static_cast<double>(clip_low), high = 1.0 + static_cast<double>(clip_high);
-            const double held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
-            const double open = ratio * adv;
-            const bool cut = open > held;   // a NaN counts as not cut and stays one
-            double kl = 0.0, g = cut ? 0.0 : -open;
-            if (ref_logp) {
-                const double u = static_cast<double>(ref_logp[col]) - lp, em = expm1(u);
-                kl = em - u;
-                if (kl_coef != 0.f) g -= static_cast<double>(kl_coef) * em;
+    __device__ Grad finish(const T& team, char*, size_t col, const ColumnSums& c, const float* x) const {
+        Grad f{};
+        if (!team.leads()) return f;
+        const double w = weight ? static_cast<double>(weight[col]) : 1.0;
+        const double adv = static_cast<double>(advantage[col]);
+        f.x = x[labels[col]];
+        const double logs = one_at_a_time(log(c.s));
+        const double lp = (static_cast<double>(f.x) - static_cast<double>(c.m)) - logs;
+        const double ratio = one_at_a_time(exp(lp - static_cast<double>(old_logp[col])));
+        const double low = 1.0 - static_cast<double>(clip_low), high = 1.0 + static_cast<double>(clip_high);
+        const double held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
+        const double open = ratio * adv;
+        const bool cut = open > held;   // a NaN counts as not cut and stays one
+        double kl = 0.0, g = cut ? 0.0 : -open;
+        double loss = -(cut ? held : open), h = 0.0;
+        if (ref_logp) {
+            const double u = static_cast<double>(ref_logp[col]) - lp, em = one_at_a_time(expm1(u));
+            kl = em - u;
+            if (kl_coef != 0.f) {
+                g -= static_cast<double>(kl_coef) * em;
+                loss += static_cast<double>(kl_coef) * kl;
             }
-            double loss = -(cut ? held : open), h = 0.0;
-            if (kl_coef != 0.f) loss += static_cast<double>(kl_coef) * kl;
-            double a = -g * w, b = 0.0;
-            if constexpr (ENTROPY) {
-                h = entropy_of(c);
-                loss -= static_cast<double>(entropy_coef) * h;
-                b = static_cast<double>(entropy_coef) * w;
-                a += b * (h - log(static_cast<double>(c.s)));
-            }
-            const double inv = 1.0 / static_cast<double>(c.s);
-            sh.g = static_cast<float>(g * w);
-            sh.x = xl;
-            sh.f = Coef{static_cast<float>(a * inv), static_cast<float>(b * inv)};
+        }
+        double a = -g * w, b = 0.0;
+        if constexpr (ENTROPY) {
+            h = logs - c.et / c.s;
+            loss -= static_cast<double>(entropy_coef) * h;
+            b = static_cast<double>(entropy_coef) * w;
+            a += b * (h - logs);
+        }
+        const double inv = 1.0 / c.s;
+        f.g = static_cast<float>(g * w);
+        f.a = static_cast<float>(a * inv);
+        f.b = static_cast<float>(b * inv);
+        if (team.rank == 0)
             write(col, static_cast<float>(lp), static_cast<float>(w * loss), static_cast<float>(w * kl),
                   cut ? static_cast<float>(w) : 0.f, static_cast<float>(w * h));
-        }
-        team.sync();
-        return sh.f;
+        return f;
     }
     template <class T>
-    __device__ void correct(const T& team, Shared& sh, size_t col, const ColumnSums& c, const Coef& f,
-                            float* out) const {
-        if (team.rank == 0) {
-            const float t = sh.x - c.m, e = exp_shifted(t, scale);
-            float v = e * f.a;
-            if constexpr (ENTROPY) v = e != 0.f ? e * (f.a + f.b * t) : 0.f;
-            out[labels[col]] = v + sh.g;
-        }
+    __device__ void correct(const T& team, char*, size_t col, float m, const Grad& f, float* out, int quads) const {
+        correct_label<ENTROPY>(team, labels[col], quads, m, f, scale, out);
     }
 };
 
@@ -107,16 +99,17 @@ JZ_API int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* sc
         return -1;
     if (kl_coef != 0.f && !ref_logp) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd);
+    float* part = scratch + kScratchFixed;
     int rc;
     if (entropy_coef != 0.f)
         rc = launch_token_kernel(PolicyHead<true>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
-                                                  scratch, clip_low, clip_high, kl_coef, entropy_coef, N},
-                                 dlogits, logits, K, N, ldx, ldg);
+                                                  part, clip_low, clip_high, kl_coef, entropy_coef, N},
+                                 scratch, dlogits, logits, K, N, ldx, ldg);
     else
         rc = launch_token_kernel(PolicyHead<false>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
-                                                   scratch, clip_low, clip_high, kl_coef, 0.f, N},
-                                 dlogits, logits, K, N, ldx, ldg);
+                                                   part, clip_low, clip_high, kl_coef, 0.f, N},
+                                 scratch, dlogits, logits, K, N, ldx, ldg);
     if (rc) return rc;
-    token_fold_kernel<float><<<4, kFoldBlock, 0, stream()>>>(sums, scratch, N, static_cast<size_t>(N), 1.0);
+    token_fold_kernel<float><<<4, kFoldBlock, 0, stream()>>>(sums, part, N, static_cast<size_t>(N), 1.0);
     return launch_rc();
 }
