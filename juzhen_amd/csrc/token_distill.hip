@@ -18,29 +18,33 @@ constexpr int kMaxTop = 512;
 
 // One of a column's entries, in LDS.
 struct Entry {
-    double lq;   // log q_j
+    double lq;   // the teacher's logit, then log q_j
     int id;      // -1: none
-    float x;     // the teacher's logit, then the student's
+    float x;     // the student's logit
 };
 
 template <bool REST>
 struct DistillHead {
-    static constexpr bool kEntropy = false, kRest = REST, kTeamwork = true, kWrites = true;
+    static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true;
+    struct Early {
+        float w;
+    };
     ExpScale scale;
     const float* teacher;
     const int32_t* ids;
     const float *lse, *weight;   // lse set iff REST; weight may be null
     float *token_loss, *part;    // token_loss may be null
-    float* picked;               // students' logits of the entries for a later kernel, or null
+    float* picked;               // the student's logits of the entries for a later kernel, or null
     size_t ldt;
     int top;
     float temperature;
 
     // entries, then one bit per logit (K = 0: the entries alone)
     __host__ __device__ size_t team_bytes(int K) const {
-        return sizeof(Entry) * static_cast<size_t>(top) + (REST ? (static_cast<size_t>(K) + 127) / 128 * 16 : 0);
+        return sizeof(Entry) * static_cast<size_t>(top) + (static_cast<size_t>(K) + 127) / 128 * 16;
     }
     __device__ unsigned* bits(char* own) const { return reinterpret_cast<unsigned*>(own + sizeof(Entry) * top); }
+    // The entries among the logits [begin, begin + len).
     template <class T>
     __device__ void mark(const T& team, unsigned* all, size_t col, int begin, int len) const {
         for (int j = team.rank; j < top; j += T::kSize) {
@@ -50,106 +54,116 @@ struct DistillHead {
     }
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
+    __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f}; }
     __device__ void write(size_t col, float each, float loss) const {
         if (token_loss) token_loss[col] = each;
         part[col] = loss;
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f); }
-    // The teacher's distribution; false where it has none.
+    // The teacher's distribution, by one wave or less; false where it has none.  all: one bit per
+    // logit, cleared, left with the entries marked (null: not kept).  x: the student's column (null:
+    // its logits at the entries are in `picked`).
     template <class T>
-    __device__ bool prologue(const T& team, char* own, size_t col, int K) const {
+    __device__ bool prologue(const T& lead, char* own, unsigned* all, size_t col, int K, const float* x) const {
         Entry* e = reinterpret_cast<Entry*>(own);
-        for (int j = team.rank; j < top; j += T::kSize) {
-            const int id = ids[col * ldt + j];
-            e[j].id = id >= 0 && id < K ? id : -1;
-            e[j].x = teacher[col * ldt + j];
-        }
-        team.sync();
+        bool twice = all == nullptr;
         float big = -INFINITY;
-        bool some = false, nan = false;
-        for (int j = team.rank; j < top; j += T::kSize) {
-            const int id = e[j].id;
-            bool keep = id >= 0;
-            for (int i = 0; i < j; ++i) keep = keep && e[i].id != id;   // an id counts once
-            e[j].lq = keep ? 1.0 : 0.0;
-            if (!keep) continue;
-            some = true;
-            nan |= e[j].x != e[j].x;
-            big = fmaxf(big, e[j].x);
+        for (int j = lead.rank; j < top; j += T::kSize) {
+            const int id = ids[col * ldt + j];
+            const bool is = id >= 0 && id < K;
+            const float t = teacher[col * ldt + j];
+            e[j].id = is ? id : -1;
+            e[j].lq = static_cast<double>(t);
+            e[j].x = !is ? 0.f : x ? x[id] : picked[col * top + j];
+            if (!is) continue;
+            big = fmaxf(big, t);
+            if (all) {
+                const unsigned bit = 1u << (id & 31);
+                twice |= (atomicOr(&all[id >> 5], bit) & bit) != 0u;
+            }
         }
-        team.sync();   // everyone has compared
-        const double T_ = static_cast<double>(temperature);
+        lead.sync();
+        if (lead.lanes(twice ? 1.f : 0.f, LargerOp{}) != 0.f) {
+            // An id counts once, the first time: the later ones are dropped.  From the back, so that
+            // each is compared with ids that are still there.
+            const int rounds = (top + T::kSize - 1) / T::kSize;
+            big = -INFINITY;
+            for (int r = rounds - 1; r >= 0; --r) {
+                const int j = lead.rank + r * T::kSize;
+                bool drop = false;
+                if (j < top)
+                    for (int i = 0; i < j; ++i) drop |= e[i].id == e[j].id;
+                lead.sync();
+                if (j < top && drop) e[j].id = -1;
+                lead.sync();
+                if (j < top && e[j].id >= 0) big = fmaxf(big, static_cast<float>(e[j].lq));
+            }
+        }
+        const double over = 1.0 / static_cast<double>(temperature);
+        float some = 0.f;
         if constexpr (REST) {
-            const double all = static_cast<double>(lse[col]);
-            for (int j = team.rank; j < top; j += T::kSize) {
-                if (e[j].lq == 0.0) e[j].id = -1;
-                e[j].lq = static_cast<double>(e[j].x) / T_ - all;
+            const double norm = static_cast<double>(lse[col]);
+            for (int j = lead.rank; j < top; j += T::kSize) {
+                e[j].lq = e[j].lq * over - norm;
+                if (e[j].id >= 0) some = 1.f;
             }
-            some = team.any(some);
+            some = lead.lanes(some, LargerOp{});
         } else {
-            big = team.max(big);
-            some = big != -INFINITY || team.any(nan);
+            big = lead.lanes(big, LargerOp{});
             double z = 0.0;
-            for (int j = team.rank; j < top; j += T::kSize) {
-                if (e[j].lq == 0.0) e[j].id = -1;
-                e[j].lq = (static_cast<double>(e[j].x) - static_cast<double>(big)) / T_;
-                if (e[j].id >= 0) z += exp(e[j].lq);
+            for (int j = lead.rank; j < top; j += T::kSize) {
+                const double t = e[j].lq, u = (t - static_cast<double>(big)) * over;
+                e[j].lq = u;
+                if (e[j].id < 0) continue;
+                z += exp64(u);
+                if (big != -INFINITY || t != t) some = 1.f;
             }
-            z = log(team.sum(z));
-            for (int j = team.rank; j < top; j += T::kSize) e[j].lq -= z;
+            z = log64(lead.lanes(z, AddOp{}));
+            some = lead.lanes(some, LargerOp{});
+            for (int j = lead.rank; j < top; j += T::kSize) e[j].lq -= z;
         }
-        return some;
+        lead.sync();
+        return some != 0.f;
     }
     template <class T>
-    __device__ Grad finish(const T& team, char* own, size_t col, const ColumnSums& c, const float* x) const {
-        Entry* e = reinterpret_cast<Entry*>(own);
-        const double T_ = static_cast<double>(temperature), logs = one_at_a_time(log(c.s));
-        const double w = weight ? static_cast<double>(weight[col]) : 1.0;
+    __device__ Grad finish(const T& lead, char* own, const Early& early, size_t col, const ColumnSums& c) const {
+        const Entry* e = reinterpret_cast<const Entry*>(own);
+        const double T_ = static_cast<double>(temperature), over = 1.0 / T_, logs = log64(c.s);
+        const double w = static_cast<double>(early.w);
         double Q = 0.0, each = 0.0;
-        for (int j = team.rank; j < top; j += T::kSize) {
+        for (int j = lead.rank; j < top; j += T::kSize) {
             if (e[j].id < 0) continue;
-            const double q = one_at_a_time(exp(e[j].lq));
-            const float xj = x[e[j].id];
-            e[j].x = xj;
-            if (picked) picked[col * top + j] = xj;
+            const double q = exp64(e[j].lq);
+            if (picked) picked[col * top + j] = e[j].x;
             Q += q;
             // an entry of no mass adds nothing, whatever the student gives it; a NaN stays one
-            if (q != 0.0) each += q * (e[j].lq - ((static_cast<double>(xj) - static_cast<double>(c.m)) / T_ - logs));
+            if (q != 0.0)
+                each += q * (e[j].lq - ((static_cast<double>(e[j].x) - static_cast<double>(c.m)) * over - logs));
         }
-        Q = team.sum(Q);
-        each = team.sum(each);
+        Q = lead.lanes(Q, AddOp{});
+        each = lead.lanes(each, AddOp{});
+        const double inv = 1.0 / c.s;
         double out = 0.0;   // what the rest subtracts
         if constexpr (REST) {
             double r = 1.0 - Q;
             r = r < 0.0 ? 0.0 : r;
-            if (r != 0.0) {
-                const double logr = one_at_a_time(log(r));
-                each += r * (logr - one_at_a_time(log(c.rest / c.s)));
-            }
+            if (r != 0.0) each += r * (log64(r) - log64(c.rest * inv));
             Q += r;
-            out = c.rest > 0.0 ? r / c.rest : Q / c.s;
+            out = c.rest > 0.0 ? r / c.rest : Q * inv;
         }
         each *= T_ * T_;
-        if (team.rank == 0) write(col, static_cast<float>(each), static_cast<float>(w * each));
-        return Grad{static_cast<float>(T_ * w * (Q / c.s - out)), 0.f, static_cast<float>(T_ * w * (Q / c.s)),
+        if (lead.rank == 0) write(col, static_cast<float>(each), static_cast<float>(w * each));
+        return Grad{static_cast<float>(T_ * w * (Q * inv - out)), 0.f, static_cast<float>(T_ * w * (Q * inv)),
                     static_cast<float>(T_ * w)};
-    }
-    // The entries of a column whose prologue has run again, as finish left them.
-    template <class T>
-    __device__ void restore(const T& team, char* own, size_t col, const Grad&) const {
-        Entry* e = reinterpret_cast<Entry*>(own);
-        for (int j = team.rank; j < top; j += T::kSize)
-            if (e[j].id >= 0) e[j].x = picked[col * top + j];
     }
     // f.g: Q*T*w/s, f.x: T*w
     template <class T>
     __device__ void correct(const T& team, char* own, size_t, float m, const Grad& f, float* out, int) const {
         const Entry* e = reinterpret_cast<const Entry*>(own);
-        team.sync();   // behind the sweep that wrote these elements as any other
-        for (int j = team.rank; j < top; j += T::kSize)
+        for (int j = team.rank; j < top; j += T::kLanes)
             if (e[j].id >= 0)
                 out[e[j].id] = exp_shifted(e[j].x - m, scale) * f.g -
-                               static_cast<float>(static_cast<double>(f.x) * exp(e[j].lq));
+                               static_cast<float>(static_cast<double>(f.x) * exp64(e[j].lq));
     }
 };
 
@@ -167,17 +181,13 @@ JZ_API int jzhip_distill_topk(float* loss_out, float* token_loss, float* dlogits
     if (!(temperature >= 1e-3f && temperature <= 1e3f)) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd), ldq = static_cast<size_t>(ldt);
     float* part = scratch + kScratchFixed;
-    float* picked = part + static_cast<size_t>(8) * N;
-    int rc;
+    float* picked = K > kMaxWhole ? part + static_cast<size_t>(8) * N : nullptr;
+    const TokenSums totals{loss_out, part, 1};
     if (teacher_lse)
-        rc = launch_token_kernel(DistillHead<true>{exp_scale(temperature), teacher, ids, teacher_lse, weight,
-                                                   token_loss, part, picked, ldq, top, temperature},
-                                 scratch, dlogits, logits, K, N, ldx, ldg);
-    else
-        rc = launch_token_kernel(DistillHead<false>{exp_scale(temperature), teacher, ids, nullptr, weight, token_loss,
-                                                    part, picked, ldq, top, temperature},
-                                 scratch, dlogits, logits, K, N, ldx, ldg);
-    if (rc) return rc;
-    token_fold_kernel<float><<<1, kFoldBlock, 0, stream()>>>(loss_out, part, N, 0, 1.0);
-    return launch_rc();
+        return launch_token_kernel(DistillHead<true>{exp_scale(temperature), teacher, ids, teacher_lse, weight,
+                                                     token_loss, part, picked, ldq, top, temperature},
+                                   totals, scratch, dlogits, logits, K, N, ldx, ldg);
+    return launch_token_kernel(DistillHead<false>{exp_scale(temperature), teacher, ids, nullptr, weight, token_loss,
+                                                  part, picked, ldq, top, temperature},
+                               totals, scratch, dlogits, logits, K, N, ldx, ldg);
 }

@@ -7,7 +7,10 @@ namespace {
 
 template <bool ENTROPY>
 struct LogprobHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeamwork = false, kWrites = false;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false;
+    struct Early {
+        float x;   // the label's logit
+    };
     ExpScale scale;
     const int32_t* labels;
     float *logp, *entropy, *stats;   // each may be null
@@ -16,8 +19,7 @@ struct LogprobHead {
     __host__ __device__ size_t team_bytes(int) const { return 0; }
     __device__ bool live(size_t col, int K) const { return label_scored(labels[col], K); }
     __device__ int label(size_t col) const { return labels[col]; }
-    template <class T>
-    __device__ bool prologue(const T&, char*, size_t, int) const { return true; }
+    __device__ Early early(size_t col, const float* x) const { return Early{x[labels[col]]}; }
     __device__ void write(size_t col, float lp, float h, float m, float s) const {
         if (logp) logp[col] = lp;
         if (ENTROPY) entropy[col] = h;
@@ -28,12 +30,10 @@ struct LogprobHead {
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f); }
     template <class T>
-    __device__ Grad finish(const T& team, char*, size_t col, const ColumnSums& c, const float* x) const {
-        if (team.leads()) {
-            const float lp = static_cast<float>(log_prob(x[labels[col]], c));
-            const float h = ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f;
-            if (team.rank == 0) write(col, lp, h, c.m, static_cast<float>(c.s));
-        }
+    __device__ Grad finish(const T& lead, char*, const Early& e, size_t col, const ColumnSums& c) const {
+        const float lp = static_cast<float>(log_prob(e.x, c));
+        const float h = ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f;
+        if (lead.rank == 0) write(col, lp, h, c.m, static_cast<float>(c.s));
         return Grad{};
     }
     template <class T>
@@ -44,13 +44,13 @@ struct LogprobHead {
 // is left, every element is read and written once.  A team of G threads takes 16*G
 // logits of a column.
 constexpr int kBwdBlock = 256, kBwdQuads = 4;
-template <int G>
+template <int G, bool NT>
 __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const float* g, const float* x,
                                                                 const int32_t* labels, const float* stats, int K,
                                                                 int N, int chunks, size_t ld, size_t ldd,
                                                                 ExpScale scale) {
     constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
-    const Team<G> team{static_cast<int>(threadIdx.x % G), nullptr};
+    const Team<G> team{static_cast<int>(threadIdx.x % G)};
     const size_t piece = static_cast<size_t>(blockIdx.x) * kTeams + threadIdx.x / G;
     const size_t col = kTeams > 1 ? piece : piece / chunks;
     if (col >= static_cast<size_t>(N)) return;
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
     const float up = g[col], m = stats[col], s = stats[static_cast<size_t>(N) + col];
     const bool live = label_scored(label, K) && s != 0.f && up != 0.f;
     if (!live) {
-        for (int q = team.rank; q < quads; q += G) *reinterpret_cast<Quad*>(out + 4 * q) = Quad(0.f);
+        for (int q = team.rank; q < quads; q += G) store_quad<NT>(out + 4 * q, Quad(0.f));
         if (team.rank < odd) out[4 * quads + team.rank] = 0.f;
         return;
     }
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
 #pragma unroll
     for (int k = 0; k < kBwdQuads; ++k) {
         const int q = team.rank + k * G;
-        if (q < quads) v[k] = *reinterpret_cast<const Quad*>(p + 4 * q);
+        if (q < quads) v[k] = load_quad<NT>(p + 4 * q);
     }
     const float last = team.rank < odd ? p[4 * quads + team.rank] : 0.f;
     const bool mine = label >= begin && label < begin + len;
@@ -85,7 +85,8 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
 #pragma unroll
     for (int k = 0; k < kBwdQuads; ++k) {
         const int q = team.rank + k * G;
-        if (q < quads) *reinterpret_cast<Quad*>(out + 4 * q) = Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)};
+        if (q < quads)
+            store_quad<NT>(out + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
     if (team.rank < odd) out[4 * quads + team.rank] = value(last);
     if (mine) correct_label<false>(team, label - begin, quads, m, f, scale, out);
@@ -94,10 +95,10 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
 int logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* x, const int32_t* labels, int K,
              int N, size_t ld) {
     if (entropy)
-        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, scratch,
-                                   nullptr, x, K, N, ld, ld);
-    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, scratch, nullptr,
-                               x, K, N, ld, ld);
+        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, TokenSums{},
+                                   scratch, nullptr, x, K, N, ld, ld);
+    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, TokenSums{}, scratch,
+                               nullptr, x, K, N, ld, ld);
 }
 
 template <int G>
@@ -106,8 +107,10 @@ int launch_bwd(float* d, const float* g, const float* x, const int32_t* labels, 
     constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
     const int chunks = kTeams > 1 ? 1 : (K + kSpan - 1) / kSpan;
     const size_t blocks = (static_cast<size_t>(N) * chunks + kTeams - 1) / kTeams;
-    logprob_bwd_kernel<G><<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N,
-                                                                                     chunks, ld, ldd, exp_scale(1.0));
+    const bool nt = streams_past_cache(static_cast<size_t>(K) * N * 2 * sizeof(float));
+    auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
+    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N, chunks, ld, ldd,
+                                                                      exp_scale(1.0));
     return launch_rc();
 }
 
@@ -135,8 +138,8 @@ __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(
     float* g, float* rewards, double* losses, const float* x, const int32_t* labels, const float* stats,
     const float* ref, PairBegins begins, int K, int N, size_t ld, int kind, float beta, float smoothing, int average,
     float scale) {
-    __shared__ double red[kPairBlock / kWave];
-    const Team<kPairBlock> team{static_cast<int>(threadIdx.x), red};
+    __shared__ double slots[4][kPairBlock / kWave];
+    const Team<kPairBlock> team{static_cast<int>(threadIdx.x)};
     const int pair = blockIdx.x;
     double reward[2], share[2];
 #pragma unroll
@@ -151,8 +154,8 @@ __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(
             gain += log_prob(x[static_cast<size_t>(n) * ld + label], c) - (ref ? static_cast<double>(ref[n]) : 0.0);
             count += 1.0;
         }
-        gain = team.sum(gain);
-        count = team.sum(count);
+        gain = team.reduce(gain, AddOp{}, slots[2 * k]);
+        count = team.reduce(count, AddOp{}, slots[2 * k + 1]);
         share[k] = average ? (count > 0.0 ? 1.0 / count : 0.0) : 1.0;
         reward[k] = static_cast<double>(beta) * gain * share[k];
     }

@@ -7,53 +7,97 @@
 // registers between the reductions, so it is read once and its gradient written once;
 // a `Head` turns (m, s, ...) into the coefficients of that gradient,
 //     d_i = e_i * (a + b*t_i)  (+ corrections at the label or the teacher's entries).
-// What bounds all of them is memory: 8 bytes per logit against about 20 vector
-// instructions (a third of what a CU issues in the time its share of 6.4 TB/s takes).
+// What bounds all of them is memory: 8 bytes per logit against about a dozen vector
+// instructions.
 //
-// Accuracy: exponentials within 0.7 ulp and without bias; a thread adds eight of them in
-// fp32 and everything further in 64 bits (two 64-bit instructions per eight elements).
+// Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.
 // Losses over many tokens cancel (the reward of an answer is a sum of small differences
-// of log-probabilities), so a bias of a few 1e-8 per token would show in them.  What
-// happens once per column (log s, ratios, divergences) is done in 64 bits too.
+// of log-probabilities), so a bias of a few 1e-8 per token would show in them: sums in
+// fp32 alone made rewards ten times less exact.  What happens once per column (log s,
+// ratios, divergences) is done in 64 bits too.
 #pragma once
 
 #include "common.hpp"
 
 #include <atomic>
+#include <cmath>
 
 namespace jz {
 
-// log2(e)/T as a sum of two floats, and the shift below which exp(d/T) < 2^-126
+// log2(e)/T as a sum of two floats, the second one positive
 struct ExpScale {
-    float hi, lo, least;
+    float hi, lo;
 };
 inline ExpScale exp_scale(double temperature) {
     const double c = 1.44269504088896340736 / temperature;
     ExpScale r;
     r.hi = static_cast<float>(c);
+    if (static_cast<double>(r.hi) >= c) r.hi = std::nextafterf(r.hi, 0.0f);
     r.lo = static_cast<float>(c - static_cast<double>(r.hi));
-    r.least = static_cast<float>(-126.0 / c);
     return r;
 }
 
-// exp(d/T) for d <= 0: 2^n * 2^f with n = rint(d*c), f = d*c - n in [-1/2, 1/2] formed by
-// fused products, 2^f by a polynomial of degree 6 (its own minimax fit of 2^f with the
-// constant term 1, relative error 2e-9, rounded coefficients: 0.67 ulp at most, mean
-// 1e-9).  Below 2^-126 the result is an exact 0, for -inf too; a NaN stays one.
+// exp(d/T) for d <= 0: the hardware's 2^u (0.7 ulp, mean error 3e-9; an exact 0 below
+// 2^-126) of u = d*log2(e)/T rounded once.  The low part of the constant is what keeps
+// the result without bias (-1.3e-8 * u otherwise); it is positive, so that d = -inf
+// gives -inf - inf and 0.  A NaN stays one.
 __device__ __forceinline__ float exp_shifted(float d, const ExpScale& c) {
-    constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer
-    const float r = fmaf(d, c.hi, kRound);
-    const float n = r - kRound;
-    const float f = fmaf(d, c.lo, fmaf(d, c.hi, -n));
-    float p = 0x1.41fbbcp-13f;
-    p = fmaf(p, f, 0x1.5f3e54p-10f);
-    p = fmaf(p, f, 0x1.3b2d4cp-7f);
-    p = fmaf(p, f, 0x1.c6aee8p-5f);
-    p = fmaf(p, f, 0x1.ebfbdcp-3f);
-    p = fmaf(p, f, 0x1.62e430p-1f);
-    p = fmaf(p, f, 1.0f);
-    p = __builtin_amdgcn_ldexpf(p, __builtin_bit_cast(int, r) - __builtin_bit_cast(int, kRound));
-    return d < c.least ? 0.0f : p;
+    return __builtin_amdgcn_exp2f(fmaf(d, c.hi, d * c.lo));
+}
+
+// ── scalars of a column, 64 bits ─────────────────────────────────────────
+// Every wave that owns a column evaluates these once, and beside 16 to 64 exponentials per
+// lane their length counts: the general library functions took longer than a column of
+// 1024 logits.  Errors stay below 1e-10 relative, a thousandth of what the sums carry.
+
+// log(v), v >= 0: v = f * 2^k with f in [1/sqrt 2, sqrt 2), log f = 2 atanh z,
+// z = (f-1)/(f+1), |z| < 0.172; the series in z^2 is cut after z^13/13.
+__device__ __forceinline__ double log64(double v) {
+    double f = __builtin_amdgcn_frexp_mant(v);   // in [1/2, 1)
+    int k = __builtin_amdgcn_frexp_exp(v);
+    const bool low = f < 0.70710678118654752;
+    f = low ? 2.0 * f : f;
+    k = low ? k - 1 : k;
+    const double z = (f - 1.0) / (f + 1.0), w = z * z;
+    double p = 1.0 / 13.0;
+    p = fma(p, w, 1.0 / 11.0);
+    p = fma(p, w, 1.0 / 9.0);
+    p = fma(p, w, 1.0 / 7.0);
+    p = fma(p, w, 1.0 / 5.0);
+    p = fma(p, w, 1.0 / 3.0);
+    p = fma(p, w, 1.0);
+    const double r = fma(static_cast<double>(k), 0.69314718055994531, 2.0 * z * p);
+    return v == 0.0 ? -INFINITY : v == INFINITY ? v : r;
+}
+// exp(v): n = rint(v/ln 2), the Taylor series of exp(v - n ln 2) up to the tenth power
+// (|r| <= 0.347: 0.347^11/11! = 2e-13).
+__device__ __forceinline__ double exp64(double v) {
+    const double n = rint(v * 1.44269504088896340736);
+    const double r = fma(n, -1.90821492927058770e-10, fma(n, -0.693147180369123816490, v));
+    double p = 1.0 / 3628800.0;
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p = __builtin_amdgcn_ldexp(p, static_cast<int>(n));
+    return v < -700.0 ? 0.0 : v > 709.0 ? INFINITY : p;
+}
+// exp(v) - 1 - v, which is v^2/2 + ... where the difference would cancel
+__device__ __forceinline__ double exp_tail64(double v) {
+    double p = 1.0 / 40320.0;
+    p = fma(p, v, 1.0 / 5040.0);
+    p = fma(p, v, 1.0 / 720.0);
+    p = fma(p, v, 1.0 / 120.0);
+    p = fma(p, v, 1.0 / 24.0);
+    p = fma(p, v, 1.0 / 6.0);
+    p = fma(p, v, 0.5) * v * v;
+    return fabs(v) < 0.06 ? p : (exp64(v) - 1.0) - v;   // 0.06^7 / 9! * 2: 1e-14
 }
 
 struct AddOp {
@@ -81,54 +125,33 @@ struct Team {
     static constexpr int kSize = G;
     static constexpr int kWaves = G > kWave ? G / kWave : 1;
     static constexpr bool kWorkgroup = kWaves > 1;
+    static constexpr int kLanes = G < kWave ? G : kWave;   // of one wave
     int rank;
-    double* red;   // 2*kWaves values, workgroup teams only
 
+    // over the team's lanes of one wave
     template <class T, class Op>
-    __device__ __forceinline__ T reduce(T v, Op op) const {
-        constexpr int W = G < kWave ? G : kWave;
-        v = op(v, dpp_mov<0xB1>(v));                          // quad_perm [1,0,3,2]
-        v = op(v, dpp_mov<0x4E>(v));                          // quad_perm [2,3,0,1]
-        if constexpr (W >= 8) v = op(v, dpp_mov<0x141>(v));   // row_half_mirror
-        if constexpr (W >= 16) v = op(v, dpp_mov<0x140>(v));  // row_mirror
-        if constexpr (W >= 32) v = op(v, __shfl_xor(v, 16, kWave));
-        if constexpr (W >= 64) v = op(v, __shfl_xor(v, 32, kWave));
+    __device__ __forceinline__ T lanes(T v, Op op) const {
+        v = op(v, dpp_mov<0xB1>(v));                               // quad_perm [1,0,3,2]
+        v = op(v, dpp_mov<0x4E>(v));                               // quad_perm [2,3,0,1]
+        if constexpr (kLanes >= 8) v = op(v, dpp_mov<0x141>(v));   // row_half_mirror
+        if constexpr (kLanes >= 16) v = op(v, dpp_mov<0x140>(v));  // row_mirror
+        if constexpr (kLanes >= 32) v = op(v, __shfl_xor(v, 16, kWave));
+        if constexpr (kLanes >= 64) v = op(v, __shfl_xor(v, 32, kWave));
+        return v;
+    }
+    // over the team; `slots`: kWaves values in LDS that nothing else uses before the next barrier
+    template <class T, class Op>
+    __device__ __forceinline__ T reduce(T v, Op op, T* slots) const {
+        v = lanes(v, op);
         if constexpr (kWorkgroup) {
-            T* slot = reinterpret_cast<T*>(red);
+            if ((rank & (kWave - 1)) == 0) slots[rank / kWave] = v;
             __syncthreads();
-            if ((rank & (kWave - 1)) == 0) slot[rank / kWave] = v;
-            __syncthreads();
-            v = slot[0];
+            v = slots[0];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) v = op(v, slot[w]);
+            for (int w = 1; w < kWaves; ++w) v = op(v, slots[w]);
         }
         return v;
     }
-    template <class T>
-    __device__ __forceinline__ T sum(T v) const { return reduce(v, AddOp{}); }
-    // two sums behind one pair of barriers
-    __device__ __forceinline__ void sum2(double& a, double& b) const {
-        Team<(G < kWave ? G : kWave)> wave{rank, nullptr};
-        a = wave.sum(a);
-        b = wave.sum(b);
-        if constexpr (kWorkgroup) {
-            __syncthreads();
-            if ((rank & (kWave - 1)) == 0) {
-                red[rank / kWave] = a;
-                red[kWaves + rank / kWave] = b;
-            }
-            __syncthreads();
-            a = red[0];
-            b = red[kWaves];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) {
-                a += red[w];
-                b += red[kWaves + w];
-            }
-        }
-    }
-    __device__ __forceinline__ float max(float v) const { return reduce(v, LargerOp{}); }
-    __device__ __forceinline__ bool any(bool v) const { return reduce(v ? 1.f : 0.f, LargerOp{}) != 0.f; }
     // LDS and global writes of the team before it are seen after it.  Lanes of one wave run
     // in step: there it only keeps the compiler from moving memory operations across.
     __device__ __forceinline__ void sync() const {
@@ -140,18 +163,11 @@ struct Team {
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
     }
-    // Work that is done once per column: by the first wave of a workgroup; by every lane of
+    // What is done once per column is done by the first wave of a workgroup; by every lane of
     // a smaller team, whose wave issues it anyway.
     __device__ __forceinline__ bool leads() const { return !kWorkgroup || rank < kWave; }
+    __device__ __forceinline__ Team<kLanes> lead() const { return Team<kLanes>{rank}; }
 };
-
-// Keeps the 64-bit functions of a column's scalars apart: interleaved they would need the
-// registers that hold the column.
-__device__ __forceinline__ double one_at_a_time(double v) {
-    asm volatile("" : "+v"(v));
-    __builtin_amdgcn_sched_barrier(0);
-    return v;
-}
 
 // What one sweep over a column leaves: its maximum, the sum of e_i, of e_i*t_i (heads
 // that ask for the entropy) and of the e_i that are none of the teacher's entries
@@ -169,13 +185,14 @@ __device__ __forceinline__ bool label_scored(int label, int K) { return label >=
 
 // log softmax of the value `x` of a column
 __device__ __forceinline__ double log_prob(float x, const ColumnSums& c) {
-    return (static_cast<double>(x) - static_cast<double>(c.m)) - log(c.s);
+    return (static_cast<double>(x) - static_cast<double>(c.m)) - log64(c.s);
 }
-__device__ __forceinline__ double entropy_of(const ColumnSums& c) { return log(c.s) - c.et / c.s; }
+__device__ __forceinline__ double entropy_of(const ColumnSums& c) { return log64(c.s) - c.et / c.s; }
 
 template <bool LINEAR>
 __device__ __forceinline__ float grad_value(float t, float e, float a, float b) {
-    if constexpr (LINEAR) return e != 0.f ? e * (a + b * t) : 0.f;
+    // (a shift of -inf goes with an exponential of 0)
+    if constexpr (LINEAR) return e * (a + b * fmaxf(t, -200.f));
     else return e * a;
 }
 
@@ -189,203 +206,90 @@ __device__ __forceinline__ unsigned known_quad(const unsigned* bits, int quad) {
 }
 __device__ __forceinline__ bool known_one(const unsigned* bits, int i) { return (bits[i >> 5] >> (i & 31)) & 1u; }
 
-// Adds fp32 values: eight (two quads) in fp32, these in 64 bits.
-struct Total {
-    double all = 0.0;
-    float open = 0.f;
-    int have = 0;
-    __device__ __forceinline__ void quad(float a, float b, float c, float d) {
-        const float q = (a + b) + (c + d);
-        if (have == 0) open = q;
-        else all += static_cast<double>(open + q);
-        have ^= 1;   // a constant in unrolled code
-    }
-    __device__ __forceinline__ double value(float last) const {
-        return all + static_cast<double>((have ? open : 0.f) + last);
-    }
+template <bool NT>
+__device__ __forceinline__ Quad load_quad(const float* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const Quad*>(p));
+    else return *reinterpret_cast<const Quad*>(p);
+}
+template <bool NT>
+__device__ __forceinline__ void store_quad(float* p, const Quad& v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<Quad*>(p));
+    else *reinterpret_cast<Quad*>(p) = v;
+}
+__device__ __forceinline__ float quad_max(const Quad& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+
+// Sums of a group of quads relative to the group's own maximum.  A thread forms them while
+// the quads behind are still on their way: exponentials need no maximum of the whole column,
+// only a factor exp(m_group - m) once that is known.
+constexpr int kGroupQuads = 4;
+struct Group {
+    float m, s, et, rest;
 };
-
-// The compiler would interleave all the independent exponentials of an unrolled loop and
-// spill what it thereby has live; where a thread holds many quads it is kept to two at a time.
-template <int NV>
-__device__ __forceinline__ void together(int k) {
-    if constexpr (NV > 4)
-        if (k % 2) __builtin_amdgcn_sched_barrier(0);
-}
-// Keeps a running sum from being formed only where it is used, its terms live until then.
-template <int NV>
-__device__ __forceinline__ void settle(Total& t, int k) {
-    if constexpr (NV > 4)
-        if (k % 2) asm volatile("" : "+v"(t.all));
-}
-
-// Columns held by teams of one wave or less (K <= 16*G, G lanes of up to four quads each) or
-// by a workgroup (K <= 4*G*(NV + NL), NV quads per thread in registers, NL in LDS).
-// A column's K % 4 last logits are one more value in the first threads of its team.
-//   dynamic LDS: NL*G quads, then per team head.team_bytes() rounded up to 16
-template <class Head, int G, int NV, int NL, int BLOCK>
-__global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, float* d, const float* x, int K, int N,
-                                                             size_t ld, size_t ldd) {
-    constexpr int kTeams = BLOCK / G;
-    __shared__ double red[2 * Team<G>::kWaves];
-    __shared__ Grad shared_grad;
-    extern __shared__ __align__(16) char dynamic[];
-    const Team<G> team{static_cast<int>(kTeams > 1 ? threadIdx.x % G : threadIdx.x), red};
-    const int slot = kTeams > 1 ? threadIdx.x / G : 0;
-    const size_t col = static_cast<size_t>(blockIdx.x) * kTeams + slot;
-    if (kTeams > 1 && col >= static_cast<size_t>(N)) return;   // whole teams
-    Quad* kept = reinterpret_cast<Quad*>(dynamic);
-    char* own = dynamic + sizeof(Quad) * NL * G + static_cast<size_t>(slot) * head.team_bytes(K);
-    const float* p = x + col * ld;
-    float* out = d ? d + col * ldd : nullptr;
-    const int quads = K / 4, odd = K % 4;
-
-    bool live = head.live(col, K);
-    Quad v[NV];
-    float last = -INFINITY;
-    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
-    if (live) {
+// x: the group's logits; without the entropy they become e_i relative to the group.  known(k): the
+// teacher's entries among quad k.
+template <class Head, class Known>
+__device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpScale& scale, Known known) {
+    Group g{-INFINITY, 0.f, 0.f, 0.f};
+    float top[kGroupQuads];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int q = team.rank + k * G;
-            v[k] = Quad(-INFINITY);
-            if (q < quads) v[k] = *reinterpret_cast<const Quad*>(p + 4 * static_cast<size_t>(q));
-        }
-        if (team.rank < odd) last = p[4 * static_cast<size_t>(quads) + team.rank];
+    for (int k = 0; k < kGroupQuads; ++k) top[k] = quad_max(x[k]);
+    g.m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    const float shift = g.m == -INFINITY ? 0.f : g.m;   // nothing but -inf: sums of 0; a NaN still shows
+    float s[kGroupQuads], et[kGroupQuads], rest[kGroupQuads];
 #pragma unroll
-        for (int k = 0; k < NL; ++k) {
-            const int q = team.rank + (NV + k) * G;
-            Quad w = Quad(-INFINITY);
-            if (q < quads) w = *reinterpret_cast<const Quad*>(p + 4 * static_cast<size_t>(q));
-            kept[k * G + team.rank] = w;
-        }
-        live = head.prologue(team, own, col, K);   // while the loads are under way
-    }
-    const unsigned* bits = nullptr;
-    if constexpr (Head::kRest) {
-        if (live) {
-            unsigned* all = head.bits(own);
-            for (int i = team.rank; i < (K + 31) / 32; i += G) all[i] = 0u;
-            team.sync();
-            head.mark(team, all, col, 0, K);
-            team.sync();
-            bits = all;
-        }
-    }
-    if (live) {
-        float m = last;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
-#pragma unroll
-        for (int k = 0; k < NL; ++k) {
-            const Quad w = kept[k * G + team.rank];
-            m = fmaxf(m, fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
-        }
-        c.m = team.max(m);
-        if (c.m == -INFINITY) {   // nothing but masked entries, or NaN
-            bool nan = last != last;
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-                nan |= v[k].x != v[k].x || v[k].y != v[k].y || v[k].z != v[k].z || v[k].w != v[k].w;
-#pragma unroll
-            for (int k = 0; k < NL; ++k) {
-                const Quad w = kept[k * G + team.rank];
-                nan |= w.x != w.x || w.y != w.y || w.z != w.z || w.w != w.w;
-            }
-            live = team.any(nan);
-        }
-    }
-    if (!live) {
-        if (team.rank == 0) head.idle(col);
-        if (out) {
-            for (int q = team.rank; q < quads; q += G) *reinterpret_cast<Quad*>(out + 4 * static_cast<size_t>(q)) = Quad(0.f);
-            if (team.rank < odd) out[4 * static_cast<size_t>(quads) + team.rank] = 0.f;
-        }
-        return;
-    }
-
-    Total s, et, rest;
-    auto add = [&](Quad& w, int q) {
-        const float t0 = w.x - c.m, t1 = w.y - c.m, t2 = w.z - c.m, t3 = w.w - c.m;
-        const float e0 = exp_shifted(t0, head.scale), e1 = exp_shifted(t1, head.scale);
-        const float e2 = exp_shifted(t2, head.scale), e3 = exp_shifted(t3, head.scale);
-        s.quad(e0, e1, e2, e3);
-        if constexpr (Head::kEntropy) {
-            et.quad(e0 != 0.f ? e0 * t0 : 0.f, e1 != 0.f ? e1 * t1 : 0.f, e2 != 0.f ? e2 * t2 : 0.f,
-                    e3 != 0.f ? e3 * t3 : 0.f);
-            w = Quad{t0, t1, t2, t3};
-        } else {
-            w = Quad{e0, e1, e2, e3};
-        }
+    for (int k = 0; k < kGroupQuads; ++k) {
+        const float t0 = x[k].x - shift, t1 = x[k].y - shift, t2 = x[k].z - shift, t3 = x[k].w - shift;
+        const float e0 = exp_shifted(t0, scale), e1 = exp_shifted(t1, scale);
+        const float e2 = exp_shifted(t2, scale), e3 = exp_shifted(t3, scale);
+        s[k] = (e0 + e1) + (e2 + e3);
+        if constexpr (Head::kEntropy)
+            et[k] = (e0 * fmaxf(t0, -200.f) + e1 * fmaxf(t1, -200.f)) + (e2 * fmaxf(t2, -200.f) + e3 * fmaxf(t3, -200.f));
+        else
+            x[k] = Quad{e0, e1, e2, e3};
         if constexpr (Head::kRest) {
-            const unsigned k = q < quads ? known_quad(bits, q) : 15u;
-            rest.quad(k & 1u ? 0.f : e0, k & 2u ? 0.f : e1, k & 4u ? 0.f : e2, k & 8u ? 0.f : e3);
+            const unsigned b = known(k);
+            rest[k] = ((b & 1u ? 0.f : e0) + (b & 2u ? 0.f : e1)) + ((b & 4u ? 0.f : e2) + (b & 8u ? 0.f : e3));
         }
-    };
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        add(v[k], team.rank + k * G);
-        if constexpr (Head::kEntropy) settle<NV>(et, k);
-        if constexpr (Head::kRest) settle<NV>(rest, k);
-        together<NV>(k);
     }
-#pragma unroll
-    for (int k = 0; k < NL; ++k) {
-        Quad w = kept[k * G + team.rank];
-        add(w, team.rank + (NV + k) * G);
-        kept[k * G + team.rank] = w;
-        if constexpr (Head::kEntropy) settle<NV>(et, k);
-        if constexpr (Head::kRest) settle<NV>(rest, k);
-        together<NV>(k);
-    }
-    const float tl = last - c.m, el = exp_shifted(tl, head.scale);
-    c.s = s.value(el);
-    if constexpr (Head::kEntropy) {
-        c.et = et.value(el != 0.f ? el * tl : 0.f);
-        team.sum2(c.s, c.et);
-    } else if constexpr (Head::kRest) {
-        c.rest = rest.value(team.rank < odd && !known_one(bits, 4 * quads + team.rank) ? el : 0.f);
-        team.sum2(c.s, c.rest);
-    } else {
-        c.s = team.sum(c.s);
-    }
-    Grad f = head.finish(team, own, col, c, p);
-    if constexpr (Team<G>::kWorkgroup && !Head::kTeamwork) {
-        if (team.rank == 0) shared_grad = f;
-        __syncthreads();
-        f = shared_grad;
-    } else {
-        team.sync();   // the gradient may replace the logits: the head has read what it needs
-    }
-    if (!Head::kWrites || !out) return;
-    auto write = [&](Quad w, int q) {
-        if (q >= quads) return;
-        Quad r;
-        if constexpr (Head::kEntropy) {
-            // the shifts are kept, not the exponentials too: those are formed again
-            asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
-            r.x = grad_value<true>(w.x, exp_shifted(w.x, head.scale), f.a, f.b);
-            r.y = grad_value<true>(w.y, exp_shifted(w.y, head.scale), f.a, f.b);
-            r.z = grad_value<true>(w.z, exp_shifted(w.z, head.scale), f.a, f.b);
-            r.w = grad_value<true>(w.w, exp_shifted(w.w, head.scale), f.a, f.b);
-        } else {
-            r = Quad{w.x * f.a, w.y * f.a, w.z * f.a, w.w * f.a};
-        }
-        *reinterpret_cast<Quad*>(out + 4 * static_cast<size_t>(q)) = r;
-    };
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        write(v[k], team.rank + k * G);
-        together<NV>(k);
-    }
-#pragma unroll
-    for (int k = 0; k < NL; ++k) {
-        write(kept[k * G + team.rank], team.rank + (NV + k) * G);
-        together<NV>(k);
-    }
-    if (team.rank < odd)
-        out[4 * static_cast<size_t>(quads) + team.rank] = grad_value<Head::kEntropy>(tl, el, f.a, f.b);
-    head.correct(team, own, col, c.m, f, out, quads);
+    g.s = (s[0] + s[1]) + (s[2] + s[3]);
+    if constexpr (Head::kEntropy) g.et = (et[0] + et[1]) + (et[2] + et[3]);
+    if constexpr (Head::kRest) g.rest = (rest[0] + rest[1]) + (rest[2] + rest[3]);
+    return g;
+}
+// Joins sums relative to two maxima (the shift of sums of nothing but -inf is 0: they are 0, or
+// NaN, and stay so).
+template <class Head>
+__device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScale& scale) {
+    if (m == -INFINITY) return;
+    const float t = c.m - m;
+    const double f = static_cast<double>(exp_shifted(t, scale));
+    if constexpr (Head::kEntropy) c.et = (c.et + c.s * static_cast<double>(fmaxf(t, -200.f))) * f;
+    if constexpr (Head::kRest) c.rest *= f;
+    c.s *= f;
+    c.m = m;
+}
+template <class Head>
+__device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
+    ColumnSums more{g.m, static_cast<double>(g.s), static_cast<double>(g.et), static_cast<double>(g.rest)};
+    const float m = fmaxf(c.m, g.m);
+    scale_sums<Head>(c, m, scale);
+    scale_sums<Head>(more, m, scale);
+    c.s += more.s;
+    if constexpr (Head::kEntropy) c.et += more.et;
+    if constexpr (Head::kRest) c.rest += more.rest;
+}
+// of a single logit
+template <class Head>
+__device__ __forceinline__ Group take_one(float x, bool known) {
+    const float e = x == -INFINITY ? 0.f : x - x + 1.f;   // exp of its shift from itself; a NaN or +inf shows
+    return Group{x, e, 0.f, known ? 0.f : e};
+}
+
+// The compiler would interleave the independent work of an unrolled loop and spill what it
+// thereby has live; where a thread holds many quads it is kept in order.
+template <int NV>
+__device__ __forceinline__ void in_order() {
+    if constexpr (NV > kGroupQuads) __builtin_amdgcn_sched_barrier(0);
 }
 
 // The label's element: the thread that wrote its quad writes it again.
@@ -399,34 +303,227 @@ __device__ __forceinline__ void correct_label(const T& team, int label, int quad
     }
 }
 
-// out[k] = scale * sum_i part[k*stride + i]: one workgroup per output, accumulated in
-// 64 bits in a fixed order.
+template <int G>
+struct ColumnShared {
+    float max[Team<G>::kWaves];
+    double s[Team<G>::kWaves], other[Team<G>::kWaves];
+    Grad grad;
+    int live;
+};
+
+// One column (K <= 4*G*(NV + NL)) by one team: NV quads per thread in registers, NL in LDS;
+// the K % 4 last logits are one more value in the first threads.
+//   own: head.team_bytes(K) of LDS, kept: NL*G quads of LDS
+template <class Head, int G, int NV, int NL, bool NT>
+__device__ __forceinline__ void token_column(const Head& head, const Team<G>& team, ColumnShared<G>& sh, char* own,
+                                             Quad* kept, size_t col, float* out, const float* p, int K) {
+    static_assert(NV % kGroupQuads == 0 && NL % kGroupQuads == 0, "whole groups");
+    constexpr int kGroups = (NV + NL) / kGroupQuads, kRegGroups = NV / kGroupQuads;
+    constexpr bool kKeepMax = Head::kWrites && !Head::kEntropy;   // the kept exponentials are relative to it
+    const int quads = K / 4, odd = K % 4;
+    bool live = head.live(col, K);
+    Quad v[kRegGroups][kGroupQuads];
+    float group_max[kGroups];
+    float last = -INFINITY;
+    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
+    typename Head::Early early{};
+    if (live) {
+        auto load = [&](int k) {
+            const int q = team.rank + k * G;
+            Quad x = Quad(-INFINITY);
+            if (q < quads) x = load_quad<NT>(p + 4 * static_cast<size_t>(q));
+            return x;
+        };
+        const unsigned* bits = nullptr;
+        auto take = [&](Quad (&x)[kGroupQuads], int i) {
+            const Group g = take_group<Head>(x, head.scale, [&](int k) {
+                const int q = team.rank + (i * kGroupQuads + k) * G;
+                return known_quad(bits, q < quads ? q : 0);   // (nothing counts behind the column)
+            });
+            add_group<Head>(c, g, head.scale);
+            if constexpr (kKeepMax) group_max[i] = g.m;
+        };
+        // The teacher's part is the first wave's and runs while the loads of the others are under
+        // way; where few registers hold the column, behind the team's own.
+        constexpr bool kTeacherFirst = Team<G>::kWorkgroup || NV > 2 * kGroupQuads;
+        auto teach = [&] {
+            if constexpr (Head::kTeacher) {
+                unsigned* marks = head.bits(own);
+                for (int i = team.rank; i < (K + 31) / 32; i += G) marks[i] = 0u;
+                team.sync();
+                if (!team.leads()) return;
+                const bool some = head.prologue(team.lead(), own, marks, col, K, p);
+                if constexpr (Team<G>::kWorkgroup) {
+                    if (team.rank == 0) sh.live = some;
+                } else {
+                    live = some;
+                }
+            }
+        };
+        if constexpr (Head::kTeacher && kTeacherFirst) teach();
+        // the quads for LDS pass through registers that the last groups use after them
+        constexpr int kFirst = NL > 0 ? NV - NL : NV;
+        Quad w[NL > 0 ? NL / kGroupQuads : 1][kGroupQuads];
+#pragma unroll
+        for (int k = 0; k < NL; ++k) w[k / kGroupQuads][k % kGroupQuads] = load(NV + k);
+#pragma unroll
+        for (int k = 0; k < kFirst; ++k) v[k / kGroupQuads][k % kGroupQuads] = load(k);
+        if (team.rank < odd) last = p[4 * static_cast<size_t>(quads) + team.rank];
+        early = head.early(col, p);
+        if constexpr (Head::kTeacher && !kTeacherFirst) teach();
+        if constexpr (Head::kRest) {
+            team.sync();   // the entries are marked
+            bits = head.bits(own);
+        }
+#pragma unroll
+        for (int i = 0; i < NL / kGroupQuads; ++i) {
+            take(w[i], kRegGroups + i);
+#pragma unroll
+            for (int k = 0; k < kGroupQuads; ++k) kept[(i * kGroupQuads + k) * G + team.rank] = w[i][k];
+            in_order<NV>();
+        }
+#pragma unroll
+        for (int k = kFirst; k < NV; ++k) v[k / kGroupQuads][k % kGroupQuads] = load(k);
+        if constexpr (NL > 0) in_order<NV>();
+#pragma unroll
+        for (int i = 0; i < kRegGroups; ++i) {
+            take(v[i], i);
+            in_order<NV>();
+        }
+        if (team.rank < odd) {
+            bool known = false;
+            if constexpr (Head::kRest) known = known_one(bits, 4 * quads + team.rank);
+            add_group<Head>(c, take_one<Head>(last, known), head.scale);
+        }
+        scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
+        if constexpr (Head::kTeacher && Team<G>::kWorkgroup) live = sh.live;   // behind that barrier
+        if constexpr (Head::kEntropy || Head::kRest) {
+            double& more = Head::kEntropy ? c.et : c.rest;
+            more = team.lanes(more, AddOp{});
+            if constexpr (Team<G>::kWorkgroup)
+                if ((team.rank & (kWave - 1)) == 0) sh.other[team.rank / kWave] = more;
+            c.s = team.reduce(c.s, AddOp{}, sh.s);
+            if constexpr (Team<G>::kWorkgroup) {
+                more = sh.other[0];
+#pragma unroll
+                for (int k = 1; k < Team<G>::kWaves; ++k) more += sh.other[k];
+            }
+        } else {
+            c.s = team.reduce(c.s, AddOp{}, sh.s);
+        }
+        live = live && !(c.m == -INFINITY && c.s == c.s);   // nothing left but masked entries; NaN counts
+    }
+    if (!live) {
+        if (team.rank == 0) head.idle(col);
+        if (Head::kWrites && out) {
+            for (int q = team.rank; q < quads; q += G) store_quad<NT>(out + 4 * static_cast<size_t>(q), Quad(0.f));
+            if (team.rank < odd) out[4 * static_cast<size_t>(quads) + team.rank] = 0.f;
+        }
+        return;
+    }
+    Grad f{};
+    if (team.leads()) f = head.finish(team.lead(), own, early, col, c);
+    if (!Head::kWrites || !out) return;
+    if constexpr (Team<G>::kWorkgroup) {
+        if (team.rank == 0) sh.grad = f;
+        __syncthreads();
+        f = sh.grad;
+    }
+    auto write = [&](const Quad& x, int q, float scale) {
+        if (q >= quads) return;
+        Quad r;
+        if constexpr (Head::kEntropy) {   // x: logits; their exponentials are formed again
+            const float t0 = x.x - c.m, t1 = x.y - c.m, t2 = x.z - c.m, t3 = x.w - c.m;
+            r.x = grad_value<true>(t0, exp_shifted(t0, head.scale), f.a, f.b);
+            r.y = grad_value<true>(t1, exp_shifted(t1, head.scale), f.a, f.b);
+            r.z = grad_value<true>(t2, exp_shifted(t2, head.scale), f.a, f.b);
+            r.w = grad_value<true>(t3, exp_shifted(t3, head.scale), f.a, f.b);
+        } else {
+            r = Quad{x.x * scale, x.y * scale, x.z * scale, x.w * scale};
+        }
+        store_quad<NT>(out + 4 * static_cast<size_t>(q), r);
+    };
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        float scale = 0.f;
+        if constexpr (kKeepMax) scale = (c.m == -INFINITY ? 1.f : exp_shifted(group_max[i] - c.m, head.scale)) * f.a;
+#pragma unroll
+        for (int k = 0; k < kGroupQuads; ++k) {
+            const int q = i * kGroupQuads + k;
+            write(i < kRegGroups ? v[i < kRegGroups ? i : 0][k] : kept[(q - NV) * G + team.rank], team.rank + q * G, scale);
+        }
+        in_order<NV>();
+    }
+    if (team.rank < odd) {
+        const float t = last - c.m;
+        out[4 * static_cast<size_t>(quads) + team.rank] = grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), f.a, f.b);
+    }
+    if constexpr (Head::kTeacher) team.sync();   // behind the sweep that wrote these elements as any other
+    if (!Head::kTeacher || team.leads()) head.correct(team, own, col, c.m, f, out, quads);
+}
+
+// out[k] = scale * sum_i part[k*stride + i] by a workgroup of BLOCK threads, in 64 bits in a fixed order.
+template <int BLOCK, class T>
+__device__ __forceinline__ void fold_parts(float* out, const T* p, int n, double scale, double* slots) {
+    const Team<BLOCK> team{static_cast<int>(threadIdx.x)};
+    double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
+    int i = team.rank;
+    for (; i + 3 * BLOCK < n; i += 4 * BLOCK) {
+        const T x0 = p[i], x1 = p[i + BLOCK], x2 = p[i + 2 * BLOCK], x3 = p[i + 3 * BLOCK];
+        a0 += static_cast<double>(x0); a1 += static_cast<double>(x1);
+        a2 += static_cast<double>(x2); a3 += static_cast<double>(x3);
+    }
+    for (; i < n; i += BLOCK) a0 += static_cast<double>(p[i]);
+    a0 = team.reduce((a0 + a1) + (a2 + a3), AddOp{}, slots);
+    if (team.rank == 0) *out = static_cast<float>(scale * a0);
+}
 constexpr int kFoldBlock = 1024;
 template <class T>
 __global__ __launch_bounds__(kFoldBlock) void token_fold_kernel(float* out, const T* part, int n, size_t stride,
                                                                 double scale) {
-    __shared__ double red[kFoldBlock / kWave];
-    const Team<kFoldBlock> team{static_cast<int>(threadIdx.x), red};
-    const T* p = part + blockIdx.x * stride;
-    double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
-    int i = team.rank;
-    for (; i + 3 * kFoldBlock < n; i += 4 * kFoldBlock) {
-        const T x0 = p[i], x1 = p[i + kFoldBlock], x2 = p[i + 2 * kFoldBlock], x3 = p[i + 3 * kFoldBlock];
-        a0 += static_cast<double>(x0); a1 += static_cast<double>(x1);
-        a2 += static_cast<double>(x2); a3 += static_cast<double>(x3);
+    __shared__ double slots[kFoldBlock / kWave];
+    fold_parts<kFoldBlock>(out + blockIdx.x, part + blockIdx.x * stride, n, scale, slots);
+}
+
+// The sums over tokens of an entry point: out[k] = sum of part[k*N ...], k < count.
+struct TokenSums {
+    float* out;
+    const float* part;
+    int count;
+};
+
+//   dynamic LDS: NL*G quads, then head.team_bytes(K) per team
+//   FOLD: a single workgroup holds all columns and adds up their parts itself
+template <class Head, int G, int NV, int NL, int BLOCK, bool NT, bool FOLD>
+__global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, TokenSums sums, float* d, const float* x,
+                                                                int K, int N, size_t ld, size_t ldd) {
+    constexpr int kTeams = BLOCK / G;
+    __shared__ ColumnShared<G> shared;
+    extern __shared__ __align__(16) char dynamic[];
+    const Team<G> team{static_cast<int>(kTeams > 1 ? threadIdx.x % G : threadIdx.x)};
+    const int slot = kTeams > 1 ? threadIdx.x / G : 0;
+    const size_t col = static_cast<size_t>(blockIdx.x) * kTeams + slot;
+    if (kTeams == 1 || col < static_cast<size_t>(N)) {   // whole teams
+        char* own = dynamic + sizeof(Quad) * NL * G + static_cast<size_t>(slot) * head.team_bytes(K);
+        token_column<Head, G, NV, NL, NT>(head, team, shared, own, reinterpret_cast<Quad*>(dynamic), col,
+                                          d ? d + col * ldd : nullptr, x + col * ld, K);
     }
-    for (; i < n; i += kFoldBlock) a0 += static_cast<double>(p[i]);
-    a0 = team.sum((a0 + a1) + (a2 + a3));
-    if (team.rank == 0) out[blockIdx.x] = static_cast<float>(scale * a0);
+    if constexpr (FOLD) {
+        __shared__ double slots[BLOCK / kWave];
+        for (int k = 0; k < sums.count; ++k) {
+            __syncthreads();   // the parts are written; the slots read
+            fold_parts<BLOCK>(sums.out + k, sums.part + static_cast<size_t>(k) * N, N, 1.0, slots);
+        }
+    }
 }
 
 // ── columns cut into chunks ──────────────────────────────────────────────
 // For columns that no workgroup holds: one workgroup per chunk leaves its
 // maximum and sums (chunk kernel), one per column joins them and makes the coefficients
-// (join), one per chunk writes the gradient (apply), where the head needs it one
+// (join), one per chunk writes the gradient (apply), where the head has a teacher one
 // per column its corrections.
-constexpr int kChunkBlock = 256, kChunkQuads = 4;
-constexpr int kChunk = 4 * kChunkBlock * kChunkQuads;
+constexpr int kChunkBlock = 256;
+constexpr int kChunk = 4 * kChunkBlock * kGroupQuads;
 struct ChunkSums {
     double s, et, rest;
     float m, pad;
@@ -446,112 +543,98 @@ static_assert(sizeof(ChunkSums) == 32 && sizeof(ColumnCoef) == 32, "scratch layo
 template <class Head>
 __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, ChunkSums* sums, const float* x, int K,
                                                                   int chunks, size_t col0, size_t ld) {
-    __shared__ double red[2 * kChunkBlock / kWave];
+    constexpr int G = kChunkBlock;
+    __shared__ ColumnShared<G> sh;
     __shared__ unsigned bits[Head::kRest ? kChunk / 32 : 1];
-    const Team<kChunkBlock> team{static_cast<int>(threadIdx.x), red};
+    const Team<G> team{static_cast<int>(threadIdx.x)};
     const int part = blockIdx.x % chunks;
     const size_t col = col0 + blockIdx.x / chunks;
     if (!head.live(col, K)) return;
     const int begin = part * kChunk, len = K - begin < kChunk ? K - begin : kChunk;
     const float* p = x + col * ld + begin;
     const int quads = len / 4, odd = len % 4;
-    Quad v[kChunkQuads];
+    Quad v[kGroupQuads];
 #pragma unroll
-    for (int k = 0; k < kChunkQuads; ++k) {
-        const int q = team.rank + k * kChunkBlock;
+    for (int k = 0; k < kGroupQuads; ++k) {
+        const int q = team.rank + k * G;
         v[k] = Quad(-INFINITY);
-        if (q < quads) v[k] = *reinterpret_cast<const Quad*>(p + 4 * q);
+        if (q < quads) v[k] = load_quad<false>(p + 4 * q);
     }
-    float last = team.rank < odd ? p[4 * quads + team.rank] : -INFINITY;
+    const float last = team.rank < odd ? p[4 * quads + team.rank] : -INFINITY;
     if constexpr (Head::kRest) {
-        for (int i = team.rank; i < kChunk / 32; i += kChunkBlock) bits[i] = 0u;
+        for (int i = team.rank; i < kChunk / 32; i += G) bits[i] = 0u;
         __syncthreads();
         head.mark(team, bits, col, begin, len);
         __syncthreads();
     }
-    float m = last;
-#pragma unroll
-    for (int k = 0; k < kChunkQuads; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
-    m = team.max(m);
-    // a chunk of -inf only: shifts of 0 - inf, sums of 0; a NaN still shows
-    const float shift = m == -INFINITY ? 0.f : m;
-    Total s, et, rest;
-    auto add = [&](float t0, float t1, float t2, float t3, unsigned known) {
-        const float e0 = exp_shifted(t0, head.scale), e1 = exp_shifted(t1, head.scale);
-        const float e2 = exp_shifted(t2, head.scale), e3 = exp_shifted(t3, head.scale);
-        s.quad(e0, e1, e2, e3);
-        if constexpr (Head::kEntropy)
-            et.quad(e0 != 0.f ? e0 * t0 : 0.f, e1 != 0.f ? e1 * t1 : 0.f, e2 != 0.f ? e2 * t2 : 0.f,
-                    e3 != 0.f ? e3 * t3 : 0.f);
-        if constexpr (Head::kRest)
-            rest.quad(known & 1u ? 0.f : e0, known & 2u ? 0.f : e1, known & 4u ? 0.f : e2, known & 8u ? 0.f : e3);
-    };
-#pragma unroll
-    for (int k = 0; k < kChunkQuads; ++k) {
-        const int q = team.rank + k * kChunkBlock;
-        add(v[k].x - shift, v[k].y - shift, v[k].z - shift, v[k].w - shift,
-            Head::kRest && q < quads ? known_quad(bits, q) : 0u);
+    const Group g = take_group<Head>(v, head.scale, [&](int k) {
+        const int q = team.rank + k * G;
+        return known_quad(bits, q < quads ? q : 0);
+    });
+    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
+    add_group<Head>(c, g, head.scale);
+    if (team.rank < odd) {
+        bool known = false;
+        if constexpr (Head::kRest) known = known_one(bits, 4 * quads + team.rank);
+        add_group<Head>(c, take_one<Head>(last, known), head.scale);
     }
-    const float tl = last - shift, el = exp_shifted(tl, head.scale);
-    ChunkSums r{0.0, 0.0, 0.0, m, 0.f};
-    r.s = s.value(el);
-    if constexpr (Head::kEntropy) {
-        r.et = et.value(el != 0.f ? el * tl : 0.f);
-        team.sum2(r.s, r.et);
-    } else if constexpr (Head::kRest) {
-        r.rest = rest.value(team.rank < odd && !known_one(bits, 4 * quads + team.rank) ? el : 0.f);
-        team.sum2(r.s, r.rest);
-    } else {
-        r.s = team.sum(r.s);
+    scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
+    double more = team.lanes(Head::kEntropy ? c.et : c.rest, AddOp{});
+    if ((team.rank & (kWave - 1)) == 0) sh.other[team.rank / kWave] = more;
+    c.s = team.reduce(c.s, AddOp{}, sh.s);
+    if (team.rank == 0) {
+        more = sh.other[0];
+        for (int w = 1; w < Team<G>::kWaves; ++w) more += sh.other[w];
+        sums[blockIdx.x] = ChunkSums{c.s, Head::kEntropy ? more : 0.0, Head::kRest ? more : 0.0, c.m, 0.f};
     }
-    if (team.rank == 0) sums[blockIdx.x] = r;
 }
 
 template <class Head>
 __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, ColumnCoef* coef, const ChunkSums* sums,
                                                                  const float* x, int K, int chunks, size_t col0,
                                                                  size_t ld) {
-    __shared__ double red[2 * kChunkBlock / kWave];
+    constexpr int G = kChunkBlock;
+    __shared__ ColumnShared<G> sh;
+    __shared__ double third[Team<G>::kWaves];
     extern __shared__ __align__(16) char dynamic[];
-    const Team<kChunkBlock> team{static_cast<int>(threadIdx.x), red};
+    const Team<G> team{static_cast<int>(threadIdx.x)};
     const size_t col = col0 + blockIdx.x;
+    const float* p = x + col * ld;
     ColumnCoef r{};
-    bool live = head.live(col, K) && head.prologue(team, dynamic, col, K);
-    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
-    if (live) {
+    bool live = head.live(col, K);
+    if (live) {   // for the whole workgroup
+        const typename Head::Early early = head.early(col, p);
+        ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
         const ChunkSums* q = sums + static_cast<size_t>(blockIdx.x) * chunks;
-        for (int i = team.rank; i < chunks; i += kChunkBlock) c.m = fmaxf(c.m, q[i].m);
-        c.m = team.max(c.m);
-        bool nan = false;
+        for (int i = team.rank; i < chunks; i += G) c.m = fmaxf(c.m, q[i].m);
+        c.m = team.reduce(c.m, LargerOp{}, sh.max);
         const double inv = static_cast<double>(head.scale.hi) + static_cast<double>(head.scale.lo);
-        for (int i = team.rank; i < chunks; i += kChunkBlock) {
+        for (int i = team.rank; i < chunks; i += G) {
             const ChunkSums w = q[i];
-            nan |= w.s != w.s;
-            if (w.m == -INFINITY) {
-                if (w.s != w.s) c.s += w.s;
-                continue;
-            }
-            const double t = static_cast<double>(w.m) - static_cast<double>(c.m);
-            const double scale = exp2(t * inv);
-            c.s += w.s * scale;
-            if (scale != 0.0) c.et += (w.et + w.s * t) * scale;
-            c.rest += w.rest * scale;
+            // a chunk of -inf adds its sums as they are: 0, or NaN
+            const double t = w.m == -INFINITY ? 0.0 : static_cast<double>(w.m) - static_cast<double>(c.m);
+            const double f = exp64(t * inv * 0.69314718055994531);
+            c.s += w.s * f;
+            c.et += (w.et + w.s * (t < -1e4 ? -1e4 : t)) * f;
+            c.rest += w.rest * f;
         }
-        c.s = team.sum(c.s);
-        if constexpr (Head::kEntropy) c.et = team.sum(c.et);
-        if constexpr (Head::kRest) c.rest = team.sum(c.rest);
-        nan = team.any(nan);
-        if (c.m == -INFINITY) live = nan;
+        c.s = team.reduce(c.s, AddOp{}, sh.s);
+        if constexpr (Head::kEntropy) c.et = team.reduce(c.et, AddOp{}, sh.other);
+        if constexpr (Head::kRest) c.rest = team.reduce(c.rest, AddOp{}, third);
+        if (!team.leads()) return;
+        live = !(c.m == -INFINITY && c.s == c.s);
+        if constexpr (Head::kTeacher) live = live && head.prologue(team.lead(), dynamic, nullptr, col, K, p);
+        if (live) {
+            r.f = head.finish(team.lead(), dynamic, early, col, c);
+            r.m = c.m;
+            r.live = 1;
+            r.label = head.label(col);
+        }
     }
-    if (live) {
-        r.f = head.finish(team, dynamic, col, c, x + col * ld);
-        r.m = c.m;
-        r.live = 1;
-        r.label = head.label(col);
-    } else if (team.rank == 0) {
-        head.idle(col);
+    if (team.rank == 0) {
+        if (!live) head.idle(col);
+        coef[blockIdx.x] = r;
     }
-    if (team.rank == 0) coef[blockIdx.x] = r;
 }
 
 template <class Head>
@@ -566,7 +649,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, flo
     float* out = d + col * ldd + begin;
     const int quads = len / 4, odd = len % 4;
     if (!r.live) {
-        for (int q = rank; q < quads; q += kChunkBlock) *reinterpret_cast<Quad*>(out + 4 * q) = Quad(0.f);
+        for (int q = rank; q < quads; q += kChunkBlock) store_quad<false>(out + 4 * q, Quad(0.f));
         if (rank < odd) out[4 * quads + rank] = 0.f;
         return;
     }
@@ -574,48 +657,47 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, flo
         const float t = y - r.m;
         return grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), r.f.a, r.f.b);
     };
-    Quad v[kChunkQuads];
+    Quad v[kGroupQuads];
 #pragma unroll
-    for (int k = 0; k < kChunkQuads; ++k) {
+    for (int k = 0; k < kGroupQuads; ++k) {
         const int q = rank + k * kChunkBlock;
-        if (q < quads) v[k] = *reinterpret_cast<const Quad*>(p + 4 * q);
+        if (q < quads) v[k] = load_quad<false>(p + 4 * q);
     }
     const float last = rank < odd ? p[4 * quads + rank] : 0.f;
 #pragma unroll
-    for (int k = 0; k < kChunkQuads; ++k) {
+    for (int k = 0; k < kGroupQuads; ++k) {
         const int q = rank + k * kChunkBlock;
-        if (q < quads) *reinterpret_cast<Quad*>(out + 4 * q) = Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)};
+        if (q < quads)
+            store_quad<false>(out + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
     if (rank < odd) out[4 * quads + rank] = value(last);
     const int label = r.label - begin;
-    if (label >= 0 && label < len) {
-        const Team<kChunkBlock> team{rank, nullptr};
-        correct_label<Head::kEntropy>(team, label, quads, r.m, r.f, head.scale, out);
-    }
+    if (label >= 0 && label < len)
+        correct_label<Head::kEntropy>(Team<kChunkBlock>{rank}, label, quads, r.m, r.f, head.scale, out);
 }
 
+// One wave per column: the teacher's entries, their gradient in its own right.
 template <class Head>
-__global__ __launch_bounds__(kChunkBlock) void token_correct_kernel(Head head, float* d, const ColumnCoef* coef, int K,
-                                                                    size_t col0, size_t ldd) {
-    __shared__ double red[2 * kChunkBlock / kWave];
+__global__ __launch_bounds__(kWave) void token_correct_kernel(Head head, float* d, const ColumnCoef* coef, int K,
+                                                              size_t col0, size_t ldd) {
     extern __shared__ __align__(16) char dynamic[];
-    const Team<kChunkBlock> team{static_cast<int>(threadIdx.x), red};
+    const Team<kWave> team{static_cast<int>(threadIdx.x)};
     const size_t col = col0 + blockIdx.x;
     const ColumnCoef r = coef[blockIdx.x];
-    if (!r.live || !head.prologue(team, dynamic, col, K)) return;
-    head.restore(team, dynamic, col, r.f);
+    if (!r.live) return;
+    head.prologue(team, dynamic, nullptr, col, K, nullptr);
     head.correct(team, dynamic, col, r.m, r.f, d + col * ldd, 0);
 }
 
 // Logits of a group of columns that are read twice: the second read comes out of the
 // 256 MB memory-side cache when they and their gradient fit it.
-constexpr size_t kGroupBytes = size_t(96) << 20;
+constexpr size_t kReadTwiceBytes = size_t(96) << 20;
 
 template <class Head>
 int launch_token_chunks(const Head& head, float* scratch, float* d, const float* x, int K, int N, size_t ld,
                         size_t ldd) {
     const int chunks = (K + kChunk - 1) / kChunk;
-    size_t group = kGroupBytes / (static_cast<size_t>(K) * sizeof(float));
+    size_t group = d ? kReadTwiceBytes / (static_cast<size_t>(K) * sizeof(float)) : static_cast<size_t>(N);
     if (group > static_cast<size_t>(kMaxChunks / chunks)) group = kMaxChunks / chunks;
     if (group > static_cast<size_t>(kMaxColumns)) group = kMaxColumns;
     if (group < 1) group = 1;
@@ -627,10 +709,11 @@ int launch_token_chunks(const Head& head, float* scratch, float* d, const float*
         const unsigned n = static_cast<unsigned>(static_cast<size_t>(N) - at < group ? static_cast<size_t>(N) - at : group);
         token_chunk_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, sums, x, K, chunks, at, ld);
         token_join_kernel<<<n, kChunkBlock, lds, st>>>(head, coef, sums, x, K, chunks, at, ld);
-        if (d) {
-            token_apply_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, d, coef, x, K, chunks, at, ld, ldd);
-            if constexpr (Head::kTeamwork)
-                token_correct_kernel<<<n, kChunkBlock, lds, st>>>(head, d, coef, K, at, ldd);
+        if constexpr (Head::kWrites) {
+            if (d) token_apply_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, d, coef, x, K, chunks, at, ld, ldd);
+        }
+        if constexpr (Head::kTeacher) {
+            if (d) token_correct_kernel<<<n, kWave, lds, st>>>(head, d, coef, K, at, ldd);
         }
         const int rc = launch_rc();
         if (rc) return rc;
@@ -638,11 +721,18 @@ int launch_token_chunks(const Head& head, float* scratch, float* d, const float*
     return 0;
 }
 
-template <class Head, int G, int NV, int NL, int BLOCK>
-int launch_token_columns(const Head& head, float* d, const float* x, int K, int N, size_t ld, size_t ldd) {
+inline int launch_token_fold(const TokenSums& sums, int N) {
+    if (sums.count == 0) return 0;
+    token_fold_kernel<float><<<sums.count, kFoldBlock, 0, stream()>>>(sums.out, sums.part, N, static_cast<size_t>(N), 1.0);
+    return launch_rc();
+}
+
+template <class Head, int G, int NV, int NL, int BLOCK, bool NT, bool FOLD>
+int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
+                            size_t ldd) {
     constexpr int kTeams = BLOCK / G;
     const size_t lds = sizeof(Quad) * NL * G + static_cast<size_t>(kTeams) * head.team_bytes(K);
-    auto kernel = token_column_kernel<Head, G, NV, NL, BLOCK>;
+    auto kernel = token_column_kernel<Head, G, NV, NL, BLOCK, NT, FOLD>;
     if (lds > (size_t(64) << 10)) {   // beyond the default limit
         static std::atomic<size_t> allowed{0};
         if (allowed.load(std::memory_order_relaxed) < lds) {
@@ -652,26 +742,45 @@ int launch_token_columns(const Head& head, float* d, const float* x, int K, int 
             allowed.store(lds, std::memory_order_relaxed);
         }
     }
-    kernel<<<(static_cast<unsigned>(N) + kTeams - 1) / kTeams, BLOCK, lds, stream()>>>(head, d, x, K, N, ld, ldd);
-    return launch_rc();
+    kernel<<<(static_cast<unsigned>(N) + kTeams - 1) / kTeams, BLOCK, lds, stream()>>>(head, sums, d, x, K, N, ld, ldd);
+    const int rc = launch_rc();
+    return rc || FOLD ? rc : launch_token_fold(sums, N);
+}
+template <class Head, int G, int NV, int NL, int BLOCK>
+int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
+                         size_t ldd) {
+    if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
+        return launch_token_columns_as<Head, G, NV, NL, BLOCK, true, false>(head, sums, d, x, K, N, ld, ldd);
+    return launch_token_columns_as<Head, G, NV, NL, BLOCK, false, false>(head, sums, d, x, K, N, ld, ldd);
+}
+// teams of one wave or less: where one workgroup holds all columns, it adds up their parts as well
+template <class Head, int G, int NV>
+int launch_token_teams(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
+                       size_t ldd) {
+    if (NV == kGroupQuads && sums.count > 0 && N <= 1024 / G)
+        return launch_token_columns_as<Head, G, kGroupQuads, 0, 1024, false, true>(head, sums, d, x, K, N, ld, ldd);
+    return launch_token_columns<Head, G, NV, 0, 256>(head, sums, d, x, K, N, ld, ldd);
 }
 
+constexpr int kMaxWhole = 131072;   // the longest column that a workgroup holds
 template <class Head>
-int launch_token_kernel(const Head& head, float* scratch, float* d, const float* x, int K, int N, size_t ld,
-                        size_t ldd) {
-    if (K <= 64) return launch_token_columns<Head, 4, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 128) return launch_token_columns<Head, 8, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 256) return launch_token_columns<Head, 16, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 512) return launch_token_columns<Head, 32, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 1024) return launch_token_columns<Head, 64, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 4096) return launch_token_columns<Head, 256, 4, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 8192) return launch_token_columns<Head, 256, 8, 0, 256>(head, d, x, K, N, ld, ldd);
-    if (K <= 16384) return launch_token_columns<Head, 512, 8, 0, 512>(head, d, x, K, N, ld, ldd);
-    if (K <= 32768) return launch_token_columns<Head, 512, 16, 0, 512>(head, d, x, K, N, ld, ldd);
-    if (K <= 65536) return launch_token_columns<Head, 1024, 16, 0, 1024>(head, d, x, K, N, ld, ldd);
-    if (K <= 98304) return launch_token_columns<Head, 1024, 24, 0, 1024>(head, d, x, K, N, ld, ldd);
-    if (K <= 131072) return launch_token_columns<Head, 1024, 24, 8, 1024>(head, d, x, K, N, ld, ldd);
-    return launch_token_chunks(head, scratch, d, x, K, N, ld, ldd);
+int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch, float* d, const float* x, int K, int N,
+                        size_t ld, size_t ldd) {
+    if (K <= 64) return launch_token_teams<Head, 4, 4>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 128) return launch_token_teams<Head, 8, 4>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 256) return launch_token_teams<Head, 16, 4>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 512) return launch_token_teams<Head, 32, 4>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 1024) return launch_token_teams<Head, 64, 4>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 2048) return launch_token_teams<Head, 64, 8>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 4096) return launch_token_teams<Head, 64, 16>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 8192) return launch_token_columns<Head, 256, 8, 0, 256>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 16384) return launch_token_columns<Head, 256, 16, 0, 256>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 32768) return launch_token_columns<Head, 512, 16, 0, 512>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 65536) return launch_token_columns<Head, 1024, 16, 0, 1024>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= 98304) return launch_token_columns<Head, 1024, 24, 0, 1024>(head, sums, d, x, K, N, ld, ldd);
+    if (K <= kMaxWhole) return launch_token_columns<Head, 1024, 24, 8, 1024>(head, sums, d, x, K, N, ld, ldd);
+    const int rc = launch_token_chunks(head, scratch, d, x, K, N, ld, ldd);
+    return rc ? rc : launch_token_fold(sums, N);
 }
 
 // The arguments every entry point of this family checks alike.

@@ -14,7 +14,10 @@ namespace {
 
 template <bool ENTROPY>
 struct PolicyHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeamwork = false, kWrites = true;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true;
+    struct Early {
+        float x, old, ref, adv, w;   // x: the label's logit
+    };
     ExpScale scale;
     const int32_t* labels;
     const float *old_logp, *ref_logp, *advantage, *weight;   // ref_logp, weight may be null
@@ -27,8 +30,10 @@ struct PolicyHead {
         return label_scored(labels[col], K) && !(weight && weight[col] == 0.f);
     }
     __device__ int label(size_t col) const { return labels[col]; }
-    template <class T>
-    __device__ bool prologue(const T&, char*, size_t, int) const { return true; }
+    __device__ Early early(size_t col, const float* x) const {
+        return Early{x[labels[col]], old_logp[col], ref_logp ? ref_logp[col] : 0.f, advantage[col],
+                     weight ? weight[col] : 1.f};
+    }
     __device__ void write(size_t col, float lp, float loss, float kl, float cut, float h) const {
         const size_t n = static_cast<size_t>(N);
         if (logp) logp[col] = lp;
@@ -39,15 +44,11 @@ struct PolicyHead {
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f, 0.f); }
     template <class T>
-    __device__ Grad finish(const T& team, char*, size_t col, const ColumnSums& c, const float* x) const {
-        Grad f{};
-        if (!team.leads()) return f;
-        const double w = weight ? static_cast<double>(weight[col]) : 1.0;
-        const double adv = static_cast<double>(advantage[col]);
-        f.x = x[labels[col]];
-        const double logs = one_at_a_time(log(c.s));
-        const double lp = (static_cast<double>(f.x) - static_cast<double>(c.m)) - logs;
-        const double ratio = one_at_a_time(exp(lp - static_cast<double>(old_logp[col])));
+    __device__ Grad finish(const T& lead, char*, const Early& e, size_t col, const ColumnSums& c) const {
+        const double w = static_cast<double>(e.w), adv = static_cast<double>(e.adv);
+        const double logs = log64(c.s);
+        const double lp = (static_cast<double>(e.x) - static_cast<double>(c.m)) - logs;
+        const double ratio = exp64(lp - static_cast<double>(e.old));
         const double low = 1.0 - static_cast<double>(clip_low), high = 1.0 + static_cast<double>(clip_high);
         const double held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
         const double open = ratio * adv;
@@ -55,28 +56,25 @@ struct PolicyHead {
         double kl = 0.0, g = cut ? 0.0 : -open;
         double loss = -(cut ? held : open), h = 0.0;
         if (ref_logp) {
-            const double u = static_cast<double>(ref_logp[col]) - lp, em = one_at_a_time(expm1(u));
-            kl = em - u;
+            const double u = static_cast<double>(e.ref) - lp;
+            kl = exp_tail64(u);
             if (kl_coef != 0.f) {
-                g -= static_cast<double>(kl_coef) * em;
+                g -= static_cast<double>(kl_coef) * (kl + u);
                 loss += static_cast<double>(kl_coef) * kl;
             }
         }
+        const double inv = 1.0 / c.s;
         double a = -g * w, b = 0.0;
         if constexpr (ENTROPY) {
-            h = logs - c.et / c.s;
+            h = logs - c.et * inv;
             loss -= static_cast<double>(entropy_coef) * h;
             b = static_cast<double>(entropy_coef) * w;
             a += b * (h - logs);
         }
-        const double inv = 1.0 / c.s;
-        f.g = static_cast<float>(g * w);
-        f.a = static_cast<float>(a * inv);
-        f.b = static_cast<float>(b * inv);
-        if (team.rank == 0)
+        if (lead.rank == 0)
             write(col, static_cast<float>(lp), static_cast<float>(w * loss), static_cast<float>(w * kl),
                   cut ? static_cast<float>(w) : 0.f, static_cast<float>(w * h));
-        return f;
+        return Grad{static_cast<float>(a * inv), static_cast<float>(b * inv), static_cast<float>(g * w), e.x};
     }
     template <class T>
     __device__ void correct(const T& team, char*, size_t col, float m, const Grad& f, float* out, int quads) const {
@@ -100,16 +98,12 @@ JZ_API int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* sc
     if (kl_coef != 0.f && !ref_logp) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd);
     float* part = scratch + kScratchFixed;
-    int rc;
+    const TokenSums totals{sums, part, 4};
     if (entropy_coef != 0.f)
-        rc = launch_token_kernel(PolicyHead<true>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
-                                                  part, clip_low, clip_high, kl_coef, entropy_coef, N},
-                                 scratch, dlogits, logits, K, N, ldx, ldg);
-    else
-        rc = launch_token_kernel(PolicyHead<false>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
-                                                   part, clip_low, clip_high, kl_coef, 0.f, N},
-                                 scratch, dlogits, logits, K, N, ldx, ldg);
-    if (rc) return rc;
-    token_fold_kernel<float><<<4, kFoldBlock, 0, stream()>>>(sums, part, N, static_cast<size_t>(N), 1.0);
-    return launch_rc();
+        return launch_token_kernel(PolicyHead<true>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight,
+                                                    logp, part, clip_low, clip_high, kl_coef, entropy_coef, N},
+                                   totals, scratch, dlogits, logits, K, N, ldx, ldg);
+    return launch_token_kernel(PolicyHead<false>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
+                                                 part, clip_low, clip_high, kl_coef, 0.f, N},
+                               totals, scratch, dlogits, logits, K, N, ldx, ldg);
 }
