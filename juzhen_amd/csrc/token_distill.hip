@@ -16,11 +16,15 @@ namespace {
 
 constexpr int kMaxTop = 512;
 
-// One of a column's entries, in LDS.
-struct Entry {
-    double lq;   // the teacher's logit, then log q_j
-    int id;      // -1: none
-    float x;     // the student's logit
+// A column's entries in LDS.
+struct Entries {
+    double* lq;   // the teacher's logit, then log q_j
+    float *q, *x;   // q_j, the student's logit
+    int* id;      // -1: none
+    static constexpr size_t kBytes = sizeof(double) + 2 * sizeof(float) + sizeof(int);
+    __device__ Entries(char* own, int top)
+        : lq(reinterpret_cast<double*>(own)), q(reinterpret_cast<float*>(lq + top)), x(q + top),
+          id(reinterpret_cast<int*>(x + top)) {}
 };
 
 template <bool REST>
@@ -28,22 +32,25 @@ struct DistillHead {
     static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true;
     struct Early {
         float w;
+        double Q;   // sum of the q_j, from the prologue
     };
     ExpScale scale;
     const float* teacher;
     const int32_t* ids;
     const float *lse, *weight;   // lse set iff REST; weight may be null
     float *token_loss, *part;    // token_loss may be null
-    float* picked;               // the student's logits of the entries for a later kernel, or null
+    float* picked;               // gradients at the entries, for a later kernel where the column is cut into chunks
     size_t ldt;
     int top;
     float temperature;
+    bool chunked = false;
 
-    // entries, then one bit per logit (K = 0: the entries alone)
+    // entries, then one bit per logit and a word more (K = 0: the entries alone)
+    __host__ __device__ size_t entry_bytes() const { return (Entries::kBytes * static_cast<size_t>(top) + 15) / 16 * 16; }
     __host__ __device__ size_t team_bytes(int K) const {
-        return sizeof(Entry) * static_cast<size_t>(top) + (static_cast<size_t>(K) + 127) / 128 * 16;
+        return entry_bytes() + (K ? (static_cast<size_t>(K) + 159) / 128 * 16 : 0);
     }
-    __device__ unsigned* bits(char* own) const { return reinterpret_cast<unsigned*>(own + sizeof(Entry) * top); }
+    __device__ unsigned* bits(char* own) const { return reinterpret_cast<unsigned*>(own + entry_bytes()); }
     // The entries among the logits [begin, begin + len).
     template <class T>
     __device__ void mark(const T& team, unsigned* all, size_t col, int begin, int len) const {
@@ -54,28 +61,28 @@ struct DistillHead {
     }
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
-    __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f}; }
+    __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, 0.0}; }
     __device__ void write(size_t col, float each, float loss) const {
         if (token_loss) token_loss[col] = each;
         part[col] = loss;
     }
     __device__ void idle(size_t col) const { write(col, 0.f, 0.f); }
     // The teacher's distribution, by one wave or less; false where it has none.  all: one bit per
-    // logit, cleared, left with the entries marked (null: not kept).  x: the student's column (null:
-    // its logits at the entries are in `picked`).
+    // logit, cleared, left with the entries marked (null: not kept).
     template <class T>
-    __device__ bool prologue(const T& lead, char* own, unsigned* all, size_t col, int K, const float* x) const {
-        Entry* e = reinterpret_cast<Entry*>(own);
+    __device__ bool prologue(const T& lead, char* own, unsigned* all, size_t col, int K, const float* x,
+                             Early& early) const {
+        const Entries e(own, top);
         bool twice = all == nullptr;
         float big = -INFINITY;
         for (int j = lead.rank; j < top; j += T::kSize) {
             const int id = ids[col * ldt + j];
             const bool is = id >= 0 && id < K;
             const float t = teacher[col * ldt + j];
-            e[j].id = is ? id : -1;
-            e[j].lq = static_cast<double>(t);
-            e[j].x = !is ? 0.f : x ? x[id] : picked[col * top + j];
+            e.id[j] = is ? id : -1;
+            e.lq[j] = static_cast<double>(t);
             if (!is) continue;
+            e.x[j] = x[id];
             big = fmaxf(big, t);
             if (all) {
                 const unsigned bit = 1u << (id & 31);
@@ -92,55 +99,66 @@ struct DistillHead {
                 const int j = lead.rank + r * T::kSize;
                 bool drop = false;
                 if (j < top)
-                    for (int i = 0; i < j; ++i) drop |= e[i].id == e[j].id;
+                    for (int i = 0; i < j; ++i) drop |= e.id[i] == e.id[j];
                 lead.sync();
-                if (j < top && drop) e[j].id = -1;
+                if (j < top && drop) e.id[j] = -1;
                 lead.sync();
-                if (j < top && e[j].id >= 0) big = fmaxf(big, static_cast<float>(e[j].lq));
+                if (j < top && e.id[j] >= 0) big = fmaxf(big, static_cast<float>(e.lq[j]));
             }
         }
         const double over = 1.0 / static_cast<double>(temperature);
         float some = 0.f;
+        double Q = 0.0;
         if constexpr (REST) {
             const double norm = static_cast<double>(lse[col]);
             for (int j = lead.rank; j < top; j += T::kSize) {
-                e[j].lq = e[j].lq * over - norm;
-                if (e[j].id >= 0) some = 1.f;
+                if (e.id[j] < 0) continue;
+                const double u = e.lq[j] * over - norm, q = exp64(u);
+                e.lq[j] = u;
+                e.q[j] = static_cast<float>(q);
+                Q += q;
+                some = 1.f;
             }
-            some = lead.lanes(some, LargerOp{});
+            Q = lead.lanes(Q, AddOp{});
         } else {
             big = lead.lanes(big, LargerOp{});
             double z = 0.0;
             for (int j = lead.rank; j < top; j += T::kSize) {
-                const double t = e[j].lq, u = (t - static_cast<double>(big)) * over;
-                e[j].lq = u;
-                if (e[j].id < 0) continue;
-                z += exp64(u);
+                if (e.id[j] < 0) continue;
+                const double t = e.lq[j], u = (t - static_cast<double>(big)) * over, q = exp64(u);
+                e.lq[j] = u;
+                e.q[j] = static_cast<float>(q);
+                z += q;
                 if (big != -INFINITY || t != t) some = 1.f;
             }
-            z = log64(lead.lanes(z, AddOp{}));
-            some = lead.lanes(some, LargerOp{});
-            for (int j = lead.rank; j < top; j += T::kSize) e[j].lq -= z;
+            z = lead.lanes(z, AddOp{});
+            const double logz = log64(z), inv = 1.0 / z;
+            for (int j = lead.rank; j < top; j += T::kSize) {
+                if (e.id[j] < 0) continue;
+                e.lq[j] -= logz;
+                e.q[j] = static_cast<float>(static_cast<double>(e.q[j]) * inv);
+            }
+            Q = z * inv;   // 1, or NaN
         }
-        lead.sync();
-        return some != 0.f;
+        early.Q = Q;
+        return lead.lanes(some, LargerOp{}) != 0.f;
+    }
+    // f.g: Q*T*w/s, f.x: T*w
+    __device__ float entry_gradient(const Entries& e, int j, float m, const Grad& f) const {
+        return exp_shifted(e.x[j] - m, scale) * f.g - f.x * e.q[j];
     }
     template <class T>
     __device__ Grad finish(const T& lead, char* own, const Early& early, size_t col, const ColumnSums& c) const {
-        const Entry* e = reinterpret_cast<const Entry*>(own);
+        const Entries e(own, top);
         const double T_ = static_cast<double>(temperature), over = 1.0 / T_, logs = log64(c.s);
         const double w = static_cast<double>(early.w);
-        double Q = 0.0, each = 0.0;
+        double Q = early.Q, each = 0.0;
         for (int j = lead.rank; j < top; j += T::kSize) {
-            if (e[j].id < 0) continue;
-            const double q = exp64(e[j].lq);
-            if (picked) picked[col * top + j] = e[j].x;
-            Q += q;
             // an entry of no mass adds nothing, whatever the student gives it; a NaN stays one
-            if (q != 0.0)
-                each += q * (e[j].lq - ((static_cast<double>(e[j].x) - static_cast<double>(c.m)) * over - logs));
+            if (e.id[j] < 0 || e.q[j] == 0.f) continue;
+            each += static_cast<double>(e.q[j]) *
+                    (e.lq[j] - ((static_cast<double>(e.x[j]) - static_cast<double>(c.m)) * over - logs));
         }
-        Q = lead.lanes(Q, AddOp{});
         each = lead.lanes(each, AddOp{});
         const double inv = 1.0 / c.s;
         double out = 0.0;   // what the rest subtracts
@@ -153,17 +171,31 @@ struct DistillHead {
         }
         each *= T_ * T_;
         if (lead.rank == 0) write(col, static_cast<float>(each), static_cast<float>(w * each));
-        return Grad{static_cast<float>(T_ * w * (Q * inv - out)), 0.f, static_cast<float>(T_ * w * (Q * inv)),
-                    static_cast<float>(T_ * w)};
+        const Grad f{static_cast<float>(T_ * w * (Q * inv - out)), 0.f, static_cast<float>(T_ * w * (Q * inv)),
+                     static_cast<float>(T_ * w)};
+        if (chunked)
+            for (int j = lead.rank; j < top; j += T::kSize)
+                if (e.id[j] >= 0) picked[col * top + j] = entry_gradient(e, j, c.m, f);
+        return f;
     }
-    // f.g: Q*T*w/s, f.x: T*w
     template <class T>
-    __device__ void correct(const T& team, char* own, size_t, float m, const Grad& f, float* out, int) const {
-        const Entry* e = reinterpret_cast<const Entry*>(own);
+    __device__ void correct(const T& team, char* own, size_t, float m, const Grad& f, float* out, const Span&) const {
+        const Entries e(own, top);
         for (int j = team.rank; j < top; j += T::kLanes)
-            if (e[j].id >= 0)
-                out[e[j].id] = exp_shifted(e[j].x - m, scale) * f.g -
-                               static_cast<float>(static_cast<double>(f.x) * exp64(e[j].lq));
+            if (e.id[j] >= 0) out[e.id[j]] = entry_gradient(e, j, m, f);
+    }
+    // The entries among the logits [begin, begin + len), whose gradients `picked` holds.
+    template <class T>
+    __device__ void correct_chunk(const T& team, char* own, size_t col, int begin, int len, float* out) const {
+        int* id = reinterpret_cast<int*>(own);
+        for (int j = team.rank; j < top; j += T::kSize) id[j] = ids[col * ldt + j];
+        team.sync();
+        for (int j = team.rank; j < top; j += T::kSize) {
+            if (id[j] < begin || id[j] >= begin + len) continue;
+            bool first = true;
+            for (int i = 0; i < j; ++i) first &= id[i] != id[j];
+            if (first) out[id[j] - begin] = picked[col * top + j];
+        }
     }
 };
 
@@ -181,7 +213,7 @@ JZ_API int jzhip_distill_topk(float* loss_out, float* token_loss, float* dlogits
     if (!(temperature >= 1e-3f && temperature <= 1e3f)) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd), ldq = static_cast<size_t>(ldt);
     float* part = scratch + kScratchFixed;
-    float* picked = K > kMaxWhole ? part + static_cast<size_t>(8) * N : nullptr;
+    float* picked = part + static_cast<size_t>(8) * N;
     const TokenSums totals{loss_out, part, 1};
     if (teacher_lse)
         return launch_token_kernel(DistillHead<true>{exp_scale(temperature), teacher, ids, teacher_lse, weight,

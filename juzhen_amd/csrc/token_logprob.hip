@@ -37,7 +37,7 @@ struct LogprobHead {
         return Grad{};
     }
     template <class T>
-    __device__ void correct(const T&, char*, size_t, float, const Grad&, float*, int) const {}
+    __device__ void correct(const T&, char*, size_t, float, const Grad&, float*, const Span&) const {}
 };
 
 // d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
@@ -56,24 +56,25 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
     if (col >= static_cast<size_t>(N)) return;
     const int begin = kTeams > 1 ? 0 : static_cast<int>(piece % chunks) * kSpan;
     const int len = K - begin < kSpan ? K - begin : kSpan;
-    const int quads = len / 4, odd = len % 4;
     const float* p = x + col * ld + begin;
     float* out = d + col * ldd + begin;
+    const Span span = span_of<(G > 4)>(out, len);
+    float* const to = out + span.skew;
     const int label = labels[col];
     const float up = g[col], m = stats[col], s = stats[static_cast<size_t>(N) + col];
     const bool live = label_scored(label, K) && s != 0.f && up != 0.f;
     if (!live) {
-        for (int q = team.rank; q < quads; q += G) store_quad<NT>(out + 4 * q, Quad(0.f));
-        if (team.rank < odd) out[4 * quads + team.rank] = 0.f;
+        for (int q = team.rank; q < span.quads; q += G) store_quad<NT>(to + 4 * q, Quad(0.f));
+        if (team.rank < span.odd) out[span.single(team.rank)] = 0.f;
         return;
     }
     Quad v[kBwdQuads];
 #pragma unroll
     for (int k = 0; k < kBwdQuads; ++k) {
         const int q = team.rank + k * G;
-        if (q < quads) v[k] = load_quad<NT>(p + 4 * q);
+        if (q < span.quads) v[k] = load_quad<NT>(p + span.skew + 4 * q);
     }
-    const float last = team.rank < odd ? p[4 * quads + team.rank] : 0.f;
+    const float last = team.rank < span.odd ? p[span.single(team.rank)] : 0.f;
     const bool mine = label >= begin && label < begin + len;
     Grad f{static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)), 0.f, up, 0.f};
     if (mine) {
@@ -85,11 +86,11 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
 #pragma unroll
     for (int k = 0; k < kBwdQuads; ++k) {
         const int q = team.rank + k * G;
-        if (q < quads)
-            store_quad<NT>(out + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
+        if (q < span.quads)
+            store_quad<NT>(to + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
-    if (team.rank < odd) out[4 * quads + team.rank] = value(last);
-    if (mine) correct_label<false>(team, label - begin, quads, m, f, scale, out);
+    if (team.rank < span.odd) out[span.single(team.rank)] = value(last);
+    if (mine) correct_label<false>(team, label - begin, span, m, f, scale, out);
 }
 
 int logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* x, const int32_t* labels, int K,

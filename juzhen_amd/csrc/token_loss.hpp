@@ -196,13 +196,34 @@ __device__ __forceinline__ float grad_value(float t, float e, float a, float b) 
     else return e * a;
 }
 
-// Four consecutive logits.  Columns start at any multiple of ld, so the address is only
-// known to be a multiple of 4 bytes; the hardware takes a 16-byte access at any of them.
+// Four consecutive logits.  Columns start at any multiple of ld, so an address is only known
+// to be a multiple of 4 bytes; the hardware takes a 16-byte access at any of them.
 typedef float Quad __attribute__((ext_vector_type(4), aligned(4)));
 
-// Which logits of a column of K belong to the teacher's entries: one bit each.
-__device__ __forceinline__ unsigned known_quad(const unsigned* bits, int quad) {
-    return (bits[quad >> 3] >> ((quad & 7) * 4)) & 15u;
+// A run of logits as `quads` quads from element `skew` on, 16-byte aligned at the address they are
+// laid out for, and `odd` single ones in front and behind (six at most).
+struct Span {
+    int skew, quads, odd;
+    __device__ __forceinline__ int single(int r) const { return r < skew ? r : 4 * quads + r; }
+    // the thread of a team of G that has element i
+    __device__ __forceinline__ int owner(int i, int G) const {
+        const int q = i < skew ? quads : (i - skew) / 4;
+        return q < quads ? q % G : i < skew ? i : i - 4 * quads;
+    }
+};
+// ALIGN: an odd leading dimension costs a wave's 1 KB access a ninth cache line otherwise.
+template <bool ALIGN>
+__device__ __forceinline__ Span span_of(const float* p, int len) {
+    int skew = ALIGN ? static_cast<int>((4 - (reinterpret_cast<uintptr_t>(p) >> 2)) & 3) : 0;
+    skew = skew < len ? skew : len;
+    const int quads = (len - skew) / 4;
+    return Span{skew, quads, len - 4 * quads};
+}
+
+// Which logits of a column belong to the teacher's entries: one bit each (one word more than
+// the last logit's is there).
+__device__ __forceinline__ unsigned known_quad(const unsigned* bits, int i) {
+    return __builtin_amdgcn_alignbit(bits[(i >> 5) + 1], bits[i >> 5], i & 31) & 15u;
 }
 __device__ __forceinline__ bool known_one(const unsigned* bits, int i) { return (bits[i >> 5] >> (i & 31)) & 1u; }
 
@@ -292,12 +313,11 @@ __device__ __forceinline__ void in_order() {
     if constexpr (NV > kGroupQuads) __builtin_amdgcn_sched_barrier(0);
 }
 
-// The label's element: the thread that wrote its quad writes it again.
+// The label's element: the thread that wrote it writes it again.
 template <bool LINEAR, class T>
-__device__ __forceinline__ void correct_label(const T& team, int label, int quads, float m, const Grad& f,
+__device__ __forceinline__ void correct_label(const T& team, int label, const Span& span, float m, const Grad& f,
                                               const ExpScale& scale, float* out) {
-    const int quad = label / 4;
-    if (team.rank == (quad < quads ? quad % T::kSize : label - 4 * quads)) {
+    if (team.rank == span.owner(label, T::kSize)) {
         const float t = f.x - m;
         out[label] = grad_value<LINEAR>(t, exp_shifted(t, scale), f.a, f.b) + f.g;
     }
@@ -311,37 +331,33 @@ struct ColumnShared {
     int live;
 };
 
-// One column (K <= 4*G*(NV + NL)) by one team: NV quads per thread in registers, NL in LDS;
-// the K % 4 last logits are one more value in the first threads.
-//   own: head.team_bytes(K) of LDS, kept: NL*G quads of LDS
-template <class Head, int G, int NV, int NL, bool NT>
+// One column by one team: NV quads per thread in registers, what is beyond them (STREAM) in tiles
+// of the same size that are read again for the gradient, the last one first: they come out of the
+// caches as long as the columns under way fit there.
+//   own: head.team_bytes(K) of LDS
+template <class Head, int G, int NV, bool NT, bool STREAM>
 __device__ __forceinline__ void token_column(const Head& head, const Team<G>& team, ColumnShared<G>& sh, char* own,
-                                             Quad* kept, size_t col, float* out, const float* p, int K) {
-    static_assert(NV % kGroupQuads == 0 && NL % kGroupQuads == 0, "whole groups");
-    constexpr int kGroups = (NV + NL) / kGroupQuads, kRegGroups = NV / kGroupQuads;
+                                             size_t col, float* out, const float* p, int K) {
+    static_assert(NV % kGroupQuads == 0, "whole groups");
+    constexpr int kGroups = NV / kGroupQuads, kTile = NV * G;
     constexpr bool kKeepMax = Head::kWrites && !Head::kEntropy;   // the kept exponentials are relative to it
-    const int quads = K / 4, odd = K % 4;
+    const Span span = span_of<(G > 4)>(p, K);   // (by the logits: values are the same bits with and without a gradient)
+    const float* const body = p + span.skew;
     bool live = head.live(col, K);
-    Quad v[kRegGroups][kGroupQuads];
+    Quad v[kGroups][kGroupQuads];
     float group_max[kGroups];
     float last = -INFINITY;
     ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
     typename Head::Early early{};
     if (live) {
-        auto load = [&](int k) {
-            const int q = team.rank + k * G;
-            Quad x = Quad(-INFINITY);
-            if (q < quads) x = load_quad<NT>(p + 4 * static_cast<size_t>(q));
-            return x;
-        };
         const unsigned* bits = nullptr;
-        auto take = [&](Quad (&x)[kGroupQuads], int i) {
+        auto take = [&](Quad (&x)[kGroupQuads], int first) {   // quads first + rank + k*G
             const Group g = take_group<Head>(x, head.scale, [&](int k) {
-                const int q = team.rank + (i * kGroupQuads + k) * G;
-                return known_quad(bits, q < quads ? q : 0);   // (nothing counts behind the column)
+                const int q = first + team.rank + k * G;
+                return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));   // (nothing counts behind the column)
             });
             add_group<Head>(c, g, head.scale);
-            if constexpr (kKeepMax) group_max[i] = g.m;
+            return g.m;
         };
         // The teacher's part is the first wave's and runs while the loads of the others are under
         // way; where few registers hold the column, behind the team's own.
@@ -352,7 +368,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
                 for (int i = team.rank; i < (K + 31) / 32; i += G) marks[i] = 0u;
                 team.sync();
                 if (!team.leads()) return;
-                const bool some = head.prologue(team.lead(), own, marks, col, K, p);
+                const bool some = head.prologue(team.lead(), own, marks, col, K, p, early);
                 if constexpr (Team<G>::kWorkgroup) {
                     if (team.rank == 0) sh.live = some;
                 } else {
@@ -360,39 +376,50 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
                 }
             }
         };
-        if constexpr (Head::kTeacher && kTeacherFirst) teach();
-        // the quads for LDS pass through registers that the last groups use after them
-        constexpr int kFirst = NL > 0 ? NV - NL : NV;
-        Quad w[NL > 0 ? NL / kGroupQuads : 1][kGroupQuads];
-#pragma unroll
-        for (int k = 0; k < NL; ++k) w[k / kGroupQuads][k % kGroupQuads] = load(NV + k);
-#pragma unroll
-        for (int k = 0; k < kFirst; ++k) v[k / kGroupQuads][k % kGroupQuads] = load(k);
-        if (team.rank < odd) last = p[4 * static_cast<size_t>(quads) + team.rank];
         early = head.early(col, p);
-        if constexpr (Head::kTeacher && !kTeacherFirst) teach();
-        if constexpr (Head::kRest) {
+        if constexpr (Head::kTeacher && kTeacherFirst) teach();
+        if constexpr (STREAM && Head::kRest) {
             team.sync();   // the entries are marked
             bits = head.bits(own);
         }
+        if constexpr (STREAM) {
+            for (int base = kTile; base < span.quads; base += kTile) {
 #pragma unroll
-        for (int i = 0; i < NL / kGroupQuads; ++i) {
-            take(w[i], kRegGroups + i);
+                for (int k = 0; k < NV; ++k) {
+                    const int q = base + team.rank + k * G;
+                    Quad& x = v[k / kGroupQuads][k % kGroupQuads];
+                    x = Quad(-INFINITY);
+                    if (q < span.quads) x = load_quad<NT && !Head::kWrites>(body + 4 * static_cast<size_t>(q));
+                }
 #pragma unroll
-            for (int k = 0; k < kGroupQuads; ++k) kept[(i * kGroupQuads + k) * G + team.rank] = w[i][k];
-            in_order<NV>();
+                for (int i = 0; i < kGroups; ++i) {
+                    take(v[i], base + i * kGroupQuads * G);
+                    in_order<NV>();
+                }
+            }
         }
 #pragma unroll
-        for (int k = kFirst; k < NV; ++k) v[k / kGroupQuads][k % kGroupQuads] = load(k);
-        if constexpr (NL > 0) in_order<NV>();
+        for (int k = 0; k < NV; ++k) {
+            const int q = team.rank + k * G;
+            Quad& x = v[k / kGroupQuads][k % kGroupQuads];
+            x = Quad(-INFINITY);
+            if (q < span.quads) x = load_quad<NT>(body + 4 * static_cast<size_t>(q));
+        }
+        if (team.rank < span.odd) last = p[span.single(team.rank)];
+        if constexpr (Head::kTeacher && !kTeacherFirst) teach();
+        if constexpr (!STREAM && Head::kRest) {
+            team.sync();
+            bits = head.bits(own);
+        }
 #pragma unroll
-        for (int i = 0; i < kRegGroups; ++i) {
-            take(v[i], i);
+        for (int i = 0; i < kGroups; ++i) {
+            const float m = take(v[i], i * kGroupQuads * G);
+            if constexpr (kKeepMax) group_max[i] = m;
             in_order<NV>();
         }
-        if (team.rank < odd) {
+        if (team.rank < span.odd) {
             bool known = false;
-            if constexpr (Head::kRest) known = known_one(bits, 4 * quads + team.rank);
+            if constexpr (Head::kRest) known = known_one(bits, span.single(team.rank));
             add_group<Head>(c, take_one<Head>(last, known), head.scale);
         }
         scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
@@ -416,8 +443,8 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     if (!live) {
         if (team.rank == 0) head.idle(col);
         if (Head::kWrites && out) {
-            for (int q = team.rank; q < quads; q += G) store_quad<NT>(out + 4 * static_cast<size_t>(q), Quad(0.f));
-            if (team.rank < odd) out[4 * static_cast<size_t>(quads) + team.rank] = 0.f;
+            for (int q = team.rank; q < span.quads; q += G) store_quad<NT>(out + span.skew + 4 * static_cast<size_t>(q), Quad(0.f));
+            if (team.rank < span.odd) out[span.single(team.rank)] = 0.f;
         }
         return;
     }
@@ -429,19 +456,10 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         __syncthreads();
         f = sh.grad;
     }
-    auto write = [&](const Quad& x, int q, float scale) {
-        if (q >= quads) return;
-        Quad r;
-        if constexpr (Head::kEntropy) {   // x: logits; their exponentials are formed again
-            const float t0 = x.x - c.m, t1 = x.y - c.m, t2 = x.z - c.m, t3 = x.w - c.m;
-            r.x = grad_value<true>(t0, exp_shifted(t0, head.scale), f.a, f.b);
-            r.y = grad_value<true>(t1, exp_shifted(t1, head.scale), f.a, f.b);
-            r.z = grad_value<true>(t2, exp_shifted(t2, head.scale), f.a, f.b);
-            r.w = grad_value<true>(t3, exp_shifted(t3, head.scale), f.a, f.b);
-        } else {
-            r = Quad{x.x * scale, x.y * scale, x.z * scale, x.w * scale};
-        }
-        store_quad<NT>(out + 4 * static_cast<size_t>(q), r);
+    float* const to = out + span.skew;
+    auto value = [&](float x) {
+        const float t = x - c.m;
+        return grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), f.a, f.b);
     };
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -449,17 +467,37 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         if constexpr (kKeepMax) scale = (c.m == -INFINITY ? 1.f : exp_shifted(group_max[i] - c.m, head.scale)) * f.a;
 #pragma unroll
         for (int k = 0; k < kGroupQuads; ++k) {
-            const int q = i * kGroupQuads + k;
-            write(i < kRegGroups ? v[i < kRegGroups ? i : 0][k] : kept[(q - NV) * G + team.rank], team.rank + q * G, scale);
+            const int q = team.rank + (i * kGroupQuads + k) * G;
+            const Quad x = v[i][k];
+            if (q >= span.quads) continue;
+            Quad r;
+            if constexpr (Head::kEntropy) r = Quad{value(x.x), value(x.y), value(x.z), value(x.w)};   // x: logits
+            else r = Quad{x.x * scale, x.y * scale, x.z * scale, x.w * scale};
+            store_quad<NT>(to + 4 * static_cast<size_t>(q), r);
         }
         in_order<NV>();
     }
-    if (team.rank < odd) {
-        const float t = last - c.m;
-        out[4 * static_cast<size_t>(quads) + team.rank] = grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), f.a, f.b);
+    if (team.rank < span.odd) out[span.single(team.rank)] = value(last);
+    if constexpr (STREAM) {
+        constexpr int kQuads = 8, kStep = kQuads * G;
+        for (int base = (span.quads - 1) / kStep * kStep; base >= kTile; base -= kStep) {
+            Quad x[kQuads];
+#pragma unroll
+            for (int k = 0; k < kQuads; ++k) {
+                const int q = base + team.rank + k * G;
+                x[k] = Quad(0.f);
+                if (q < span.quads) x[k] = load_quad<NT>(body + 4 * static_cast<size_t>(q));
+            }
+#pragma unroll
+            for (int k = 0; k < kQuads; ++k) {
+                const int q = base + team.rank + k * G;
+                const Quad r{value(x[k].x), value(x[k].y), value(x[k].z), value(x[k].w)};
+                if (q < span.quads) store_quad<NT>(to + 4 * static_cast<size_t>(q), r);
+            }
+        }
     }
     if constexpr (Head::kTeacher) team.sync();   // behind the sweep that wrote these elements as any other
-    if (!Head::kTeacher || team.leads()) head.correct(team, own, col, c.m, f, out, quads);
+    if (!Head::kTeacher || team.leads()) head.correct(team, own, col, c.m, f, out, span);
 }
 
 // out[k] = scale * sum_i part[k*stride + i] by a workgroup of BLOCK threads, in 64 bits in a fixed order.
@@ -492,9 +530,9 @@ struct TokenSums {
     int count;
 };
 
-//   dynamic LDS: NL*G quads, then head.team_bytes(K) per team
+//   dynamic LDS: head.team_bytes(K) per team
 //   FOLD: a single workgroup holds all columns and adds up their parts itself
-template <class Head, int G, int NV, int NL, int BLOCK, bool NT, bool FOLD>
+template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
 __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, TokenSums sums, float* d, const float* x,
                                                                 int K, int N, size_t ld, size_t ldd) {
     constexpr int kTeams = BLOCK / G;
@@ -504,9 +542,8 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
     const int slot = kTeams > 1 ? threadIdx.x / G : 0;
     const size_t col = static_cast<size_t>(blockIdx.x) * kTeams + slot;
     if (kTeams == 1 || col < static_cast<size_t>(N)) {   // whole teams
-        char* own = dynamic + sizeof(Quad) * NL * G + static_cast<size_t>(slot) * head.team_bytes(K);
-        token_column<Head, G, NV, NL, NT>(head, team, shared, own, reinterpret_cast<Quad*>(dynamic), col,
-                                          d ? d + col * ldd : nullptr, x + col * ld, K);
+        token_column<Head, G, NV, NT, STREAM>(head, team, shared, dynamic + static_cast<size_t>(slot) * head.team_bytes(K),
+                                              col, d ? d + col * ldd : nullptr, x + col * ld, K);
     }
     if constexpr (FOLD) {
         __shared__ double slots[BLOCK / kWave];
@@ -520,8 +557,7 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
 // ── columns cut into chunks ──────────────────────────────────────────────
 // For columns that no workgroup holds: one workgroup per chunk leaves its
 // maximum and sums (chunk kernel), one per column joins them and makes the coefficients
-// (join), one per chunk writes the gradient (apply), where the head has a teacher one
-// per column its corrections.
+// (join), one per chunk writes the gradient (apply).
 constexpr int kChunkBlock = 256;
 constexpr int kChunk = 4 * kChunkBlock * kGroupQuads;
 struct ChunkSums {
@@ -545,22 +581,22 @@ __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, Chu
                                                                   int chunks, size_t col0, size_t ld) {
     constexpr int G = kChunkBlock;
     __shared__ ColumnShared<G> sh;
-    __shared__ unsigned bits[Head::kRest ? kChunk / 32 : 1];
+    __shared__ unsigned bits[Head::kRest ? kChunk / 32 + 1 : 1];
     const Team<G> team{static_cast<int>(threadIdx.x)};
     const int part = blockIdx.x % chunks;
     const size_t col = col0 + blockIdx.x / chunks;
     if (!head.live(col, K)) return;
     const int begin = part * kChunk, len = K - begin < kChunk ? K - begin : kChunk;
     const float* p = x + col * ld + begin;
-    const int quads = len / 4, odd = len % 4;
+    const Span span = span_of<true>(p, len);
     Quad v[kGroupQuads];
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) {
         const int q = team.rank + k * G;
         v[k] = Quad(-INFINITY);
-        if (q < quads) v[k] = load_quad<false>(p + 4 * q);
+        if (q < span.quads) v[k] = load_quad<false>(p + span.skew + 4 * q);
     }
-    const float last = team.rank < odd ? p[4 * quads + team.rank] : -INFINITY;
+    const float last = team.rank < span.odd ? p[span.single(team.rank)] : -INFINITY;
     if constexpr (Head::kRest) {
         for (int i = team.rank; i < kChunk / 32; i += G) bits[i] = 0u;
         __syncthreads();
@@ -569,13 +605,13 @@ __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, Chu
     }
     const Group g = take_group<Head>(v, head.scale, [&](int k) {
         const int q = team.rank + k * G;
-        return known_quad(bits, q < quads ? q : 0);
+        return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));
     });
     ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
     add_group<Head>(c, g, head.scale);
-    if (team.rank < odd) {
+    if (team.rank < span.odd) {
         bool known = false;
-        if constexpr (Head::kRest) known = known_one(bits, 4 * quads + team.rank);
+        if constexpr (Head::kRest) known = known_one(bits, span.single(team.rank));
         add_group<Head>(c, take_one<Head>(last, known), head.scale);
     }
     scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
@@ -603,7 +639,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
     ColumnCoef r{};
     bool live = head.live(col, K);
     if (live) {   // for the whole workgroup
-        const typename Head::Early early = head.early(col, p);
+        typename Head::Early early = head.early(col, p);
         ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
         const ChunkSums* q = sums + static_cast<size_t>(blockIdx.x) * chunks;
         for (int i = team.rank; i < chunks; i += G) c.m = fmaxf(c.m, q[i].m);
@@ -623,7 +659,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
         if constexpr (Head::kRest) c.rest = team.reduce(c.rest, AddOp{}, third);
         if (!team.leads()) return;
         live = !(c.m == -INFINITY && c.s == c.s);
-        if constexpr (Head::kTeacher) live = live && head.prologue(team.lead(), dynamic, nullptr, col, K, p);
+        if constexpr (Head::kTeacher) live = live && head.prologue(team.lead(), dynamic, nullptr, col, K, p, early);
         if (live) {
             r.f = head.finish(team.lead(), dynamic, early, col, c);
             r.m = c.m;
@@ -638,19 +674,28 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
 }
 
 template <class Head>
-__global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, float* d, const ColumnCoef* coef,
-                                                                  const float* x, int K, int chunks, size_t col0,
-                                                                  size_t ld, size_t ldd) {
+__global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, TokenSums sums, float* d,
+                                                                  const ColumnCoef* coef, const float* x, int K, int N,
+                                                                  int chunks, size_t col0, size_t ld, size_t ldd) {
+    __shared__ double slots[kChunkBlock / kWave];
+    extern __shared__ __align__(16) char dynamic[];
     const int rank = threadIdx.x, part = blockIdx.x % chunks;
+    if (blockIdx.x == 0)   // every column is joined: the last group's first workgroup adds up their parts
+        for (int k = 0; k < sums.count; ++k) {
+            fold_parts<kChunkBlock>(sums.out + k, sums.part + static_cast<size_t>(k) * N, N, 1.0, slots);
+            __syncthreads();
+        }
     const size_t col = col0 + blockIdx.x / chunks;
     const ColumnCoef r = coef[blockIdx.x / chunks];
     const int begin = part * kChunk, len = K - begin < kChunk ? K - begin : kChunk;
     const float* p = x + col * ld + begin;
     float* out = d + col * ldd + begin;
-    const int quads = len / 4, odd = len % 4;
+    const Span span = span_of<true>(out, len);
+    p += span.skew;
+    float* const to = out + span.skew;
     if (!r.live) {
-        for (int q = rank; q < quads; q += kChunkBlock) store_quad<false>(out + 4 * q, Quad(0.f));
-        if (rank < odd) out[4 * quads + rank] = 0.f;
+        for (int q = rank; q < span.quads; q += kChunkBlock) store_quad<false>(to + 4 * q, Quad(0.f));
+        if (rank < span.odd) out[span.single(rank)] = 0.f;
         return;
     }
     auto value = [&](float y) {
@@ -661,65 +706,28 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, flo
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) {
         const int q = rank + k * kChunkBlock;
-        if (q < quads) v[k] = load_quad<false>(p + 4 * q);
+        if (q < span.quads) v[k] = load_quad<false>(p + 4 * q);
     }
-    const float last = rank < odd ? p[4 * quads + rank] : 0.f;
+    const float last = rank < span.odd ? p[span.single(rank) - span.skew] : 0.f;
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) {
         const int q = rank + k * kChunkBlock;
-        if (q < quads)
-            store_quad<false>(out + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
+        if (q < span.quads)
+            store_quad<false>(to + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
-    if (rank < odd) out[4 * quads + rank] = value(last);
+    if (rank < span.odd) out[span.single(rank)] = value(last);
     const int label = r.label - begin;
     if (label >= 0 && label < len)
-        correct_label<Head::kEntropy>(Team<kChunkBlock>{rank}, label, quads, r.m, r.f, head.scale, out);
-}
-
-// One wave per column: the teacher's entries, their gradient in its own right.
-template <class Head>
-__global__ __launch_bounds__(kWave) void token_correct_kernel(Head head, float* d, const ColumnCoef* coef, int K,
-                                                              size_t col0, size_t ldd) {
-    extern __shared__ __align__(16) char dynamic[];
-    const Team<kWave> team{static_cast<int>(threadIdx.x)};
-    const size_t col = col0 + blockIdx.x;
-    const ColumnCoef r = coef[blockIdx.x];
-    if (!r.live) return;
-    head.prologue(team, dynamic, nullptr, col, K, nullptr);
-    head.correct(team, dynamic, col, r.m, r.f, d + col * ldd, 0);
+        correct_label<Head::kEntropy>(Team<kChunkBlock>{rank}, label, span, r.m, r.f, head.scale, out);
+    if constexpr (Head::kTeacher) {
+        __syncthreads();   // behind the sweep that wrote these elements as any other
+        head.correct_chunk(Team<kChunkBlock>{rank}, dynamic, col, begin, len, out);
+    }
 }
 
 // Logits of a group of columns that are read twice: the second read comes out of the
 // 256 MB memory-side cache when they and their gradient fit it.
 constexpr size_t kReadTwiceBytes = size_t(96) << 20;
-
-template <class Head>
-int launch_token_chunks(const Head& head, float* scratch, float* d, const float* x, int K, int N, size_t ld,
-                        size_t ldd) {
-    const int chunks = (K + kChunk - 1) / kChunk;
-    size_t group = d ? kReadTwiceBytes / (static_cast<size_t>(K) * sizeof(float)) : static_cast<size_t>(N);
-    if (group > static_cast<size_t>(kMaxChunks / chunks)) group = kMaxChunks / chunks;
-    if (group > static_cast<size_t>(kMaxColumns)) group = kMaxColumns;
-    if (group < 1) group = 1;
-    ChunkSums* sums = reinterpret_cast<ChunkSums*>(scratch);
-    ColumnCoef* coef = reinterpret_cast<ColumnCoef*>(scratch + kScratchFixed / 2);
-    const size_t lds = head.team_bytes(0);
-    hipStream_t st = stream();
-    for (size_t at = 0; at < static_cast<size_t>(N); at += group) {
-        const unsigned n = static_cast<unsigned>(static_cast<size_t>(N) - at < group ? static_cast<size_t>(N) - at : group);
-        token_chunk_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, sums, x, K, chunks, at, ld);
-        token_join_kernel<<<n, kChunkBlock, lds, st>>>(head, coef, sums, x, K, chunks, at, ld);
-        if constexpr (Head::kWrites) {
-            if (d) token_apply_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, d, coef, x, K, chunks, at, ld, ldd);
-        }
-        if constexpr (Head::kTeacher) {
-            if (d) token_correct_kernel<<<n, kWave, lds, st>>>(head, d, coef, K, at, ldd);
-        }
-        const int rc = launch_rc();
-        if (rc) return rc;
-    }
-    return 0;
-}
 
 inline int launch_token_fold(const TokenSums& sums, int N) {
     if (sums.count == 0) return 0;
@@ -727,12 +735,41 @@ inline int launch_token_fold(const TokenSums& sums, int N) {
     return launch_rc();
 }
 
-template <class Head, int G, int NV, int NL, int BLOCK, bool NT, bool FOLD>
+template <class Head>
+int launch_token_chunks(Head head, const TokenSums& sums, float* scratch, float* d, const float* x, int K, int N,
+                        size_t ld, size_t ldd) {
+    const int chunks = (K + kChunk - 1) / kChunk;
+    size_t group = Head::kWrites ? kReadTwiceBytes / (static_cast<size_t>(K) * sizeof(float)) : static_cast<size_t>(N);
+    if (group > static_cast<size_t>(kMaxChunks / chunks)) group = kMaxChunks / chunks;
+    if (group > static_cast<size_t>(kMaxColumns)) group = kMaxColumns;
+    if (group < 1) group = 1;
+    ChunkSums* part = reinterpret_cast<ChunkSums*>(scratch);
+    ColumnCoef* coef = reinterpret_cast<ColumnCoef*>(scratch + kScratchFixed / 2);
+    const size_t lds = head.team_bytes(0);
+    if constexpr (Head::kTeacher) head.chunked = true;
+    hipStream_t st = stream();
+    for (size_t at = 0; at < static_cast<size_t>(N); at += group) {
+        const bool last = static_cast<size_t>(N) - at <= group;
+        const unsigned n = static_cast<unsigned>(last ? static_cast<size_t>(N) - at : group);
+        token_chunk_kernel<<<n * chunks, kChunkBlock, 0, st>>>(head, part, x, K, chunks, at, ld);
+        token_join_kernel<<<n, kChunkBlock, lds, st>>>(head, coef, part, x, K, chunks, at, ld);
+        if constexpr (Head::kWrites) {
+            if (d)
+                token_apply_kernel<<<n * chunks, kChunkBlock, lds, st>>>(head, last ? sums : TokenSums{}, d, coef, x, K, N,
+                                                                         chunks, at, ld, ldd);
+        }
+        const int rc = launch_rc();
+        if (rc) return rc;
+    }
+    return d ? 0 : launch_token_fold(sums, N);
+}
+
+template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
 int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                             size_t ldd) {
     constexpr int kTeams = BLOCK / G;
-    const size_t lds = sizeof(Quad) * NL * G + static_cast<size_t>(kTeams) * head.team_bytes(K);
-    auto kernel = token_column_kernel<Head, G, NV, NL, BLOCK, NT, FOLD>;
+    const size_t lds = static_cast<size_t>(kTeams) * head.team_bytes(K);
+    auto kernel = token_column_kernel<Head, G, NV, BLOCK, NT, STREAM, FOLD>;
     if (lds > (size_t(64) << 10)) {   // beyond the default limit
         static std::atomic<size_t> allowed{0};
         if (allowed.load(std::memory_order_relaxed) < lds) {
@@ -746,23 +783,32 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
     const int rc = launch_rc();
     return rc || FOLD ? rc : launch_token_fold(sums, N);
 }
-template <class Head, int G, int NV, int NL, int BLOCK>
+template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                          size_t ldd) {
     if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
-        return launch_token_columns_as<Head, G, NV, NL, BLOCK, true, false>(head, sums, d, x, K, N, ld, ldd);
-    return launch_token_columns_as<Head, G, NV, NL, BLOCK, false, false>(head, sums, d, x, K, N, ld, ldd);
+        return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
+    return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }
 // teams of one wave or less: where one workgroup holds all columns, it adds up their parts as well
 template <class Head, int G, int NV>
 int launch_token_teams(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                        size_t ldd) {
-    if (NV == kGroupQuads && sums.count > 0 && N <= 1024 / G)
-        return launch_token_columns_as<Head, G, kGroupQuads, 0, 1024, false, true>(head, sums, d, x, K, N, ld, ldd);
-    return launch_token_columns<Head, G, NV, 0, 256>(head, sums, d, x, K, N, ld, ldd);
+    if (NV == kGroupQuads && sums.count > 0 && N <= 1024 / G && (1024 / G) * head.team_bytes(K) <= (size_t(64) << 10))
+        return launch_token_columns_as<Head, G, kGroupQuads, 1024, false, false, true>(head, sums, d, x, K, N, ld, ldd);
+    return launch_token_columns<Head, G, NV, 256, false>(head, sums, d, x, K, N, ld, ldd);
 }
 
-constexpr int kMaxWhole = 131072;   // the longest column that a workgroup holds
+// Which way a call goes.  us on MI355X, 512 MB of logits (a quarter of the tokens unscored) unless said
+// otherwise; "values": logprobs, "gradient": the policy loss.
+constexpr int kMaxTeam = 4096, kMaxResident = 32768;
+constexpr size_t kMaxLds = size_t(150) << 10;   // of 160 KB, beside what the kernels declare themselves
+inline bool token_in_chunks(int K, int N, bool gradient) {
+    // A few long columns occupy as many CUs: 1 x 262144 values 25 -> 7, gradient 41 -> 14; 64 x 131072
+    // 15 -> 8.5 and 25 -> 19.  With more columns the second read of the gradient decides: 128 x 262144 gradient
+    // 56 in one piece, 63 in chunks; values 28 and 21, 256 x 262144 36 and 34.
+    return K > 2 * kMaxResident && static_cast<long long>(N) * (gradient ? 4 : 2) <= num_cus();
+}
 template <class Head>
 int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch, float* d, const float* x, int K, int N,
                         size_t ld, size_t ldd) {
@@ -772,15 +818,28 @@ int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch,
     if (K <= 512) return launch_token_teams<Head, 32, 4>(head, sums, d, x, K, N, ld, ldd);
     if (K <= 1024) return launch_token_teams<Head, 64, 4>(head, sums, d, x, K, N, ld, ldd);
     if (K <= 2048) return launch_token_teams<Head, 64, 8>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 4096) return launch_token_teams<Head, 64, 16>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 8192) return launch_token_columns<Head, 256, 8, 0, 256>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 16384) return launch_token_columns<Head, 256, 16, 0, 256>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 32768) return launch_token_columns<Head, 512, 16, 0, 512>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 65536) return launch_token_columns<Head, 1024, 16, 0, 1024>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= 98304) return launch_token_columns<Head, 1024, 24, 0, 1024>(head, sums, d, x, K, N, ld, ldd);
-    if (K <= kMaxWhole) return launch_token_columns<Head, 1024, 24, 8, 1024>(head, sums, d, x, K, N, ld, ldd);
-    const int rc = launch_token_chunks(head, scratch, d, x, K, N, ld, ldd);
-    return rc ? rc : launch_token_fold(sums, N);
+    if (K <= kMaxTeam) return launch_token_teams<Head, 64, 16>(head, sums, d, x, K, N, ld, ldd);
+    if (token_in_chunks(K, N, Head::kWrites) || head.team_bytes(K) > kMaxLds) return launch_token_chunks(head, sums, scratch, d, x, K, N, ld, ldd);
+    if (K <= 8192) return launch_token_columns<Head, 256, 8, 256, false>(head, sums, d, x, K, N, ld, ldd);
+    if constexpr (!Head::kWrites) {
+        // Values alone need no column kept; small tiles waste least of their last round: K = 24000 61 (512 x 16
+        // quads in one tile: 68), 131072 65 (1024 x 24 quads: 90).
+        if (K <= 2 * 8192) return launch_token_columns<Head, 256, 4, 256, true>(head, sums, d, x, K, N, ld, ldd);
+        return launch_token_columns<Head, 512, 4, 512, true>(head, sums, d, x, K, N, ld, ldd);
+    } else {
+        if (K <= 16384) return launch_token_columns<Head, 256, 16, 256, false>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= kMaxResident) return launch_token_columns<Head, 512, 16, 512, false>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 2 * kMaxResident) {
+            // Half of the column kept and two workgroups on a CU, whose loads and stores overlap: K = 48000 158
+            // (one workgroup that keeps all of it: 177), 64000 168 (169), with the teacher's rest 187 (237).  Where
+            // there is no second workgroup, the one: 256 x 64000 22 (25).
+            if (N > 2 * num_cus()) return launch_token_columns<Head, 512, 16, 512, true>(head, sums, d, x, K, N, ld, ldd);
+            return launch_token_columns<Head, 1024, 16, 1024, false>(head, sums, d, x, K, N, ld, ldd);
+        }
+        // K = 98000 171 (512 threads: 197; 24 quads: 183), 262144 193 (215; 191), rest 230 (239; 248); chunks read
+        // twice over several launches 280.
+        return launch_token_columns<Head, 1024, 16, 1024, true>(head, sums, d, x, K, N, ld, ldd);
+    }
 }
 
 // The arguments every entry point of this family checks alike.
