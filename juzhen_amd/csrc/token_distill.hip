@@ -59,6 +59,7 @@ struct DistillHead {
             if (at >= begin && at < begin + len) atomicOr(&all[(at - begin) >> 5], 1u << ((at - begin) & 31));
         }
     }
+    bool read_again() const { return false; }
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
     __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, 0.0}; }

@@ -15,23 +15,26 @@ struct LogprobHead {
     const int32_t* labels;
     float *logp, *entropy, *stats;   // each may be null
     int N;
+    double* exact;                   // log p once more for a loss over many tokens, or null
 
     __host__ __device__ size_t team_bytes(int) const { return 0; }
+    bool read_again() const { return exact != nullptr; }   // the gradient's sweep follows: leave the caches be
     __device__ bool live(size_t col, int K) const { return label_scored(labels[col], K); }
     __device__ int label(size_t col) const { return labels[col]; }
     __device__ Early early(size_t col, const float* x) const { return Early{x[labels[col]]}; }
-    __device__ void write(size_t col, float lp, float h, float m, float s) const {
-        if (logp) logp[col] = lp;
+    __device__ void write(size_t col, double lp, float h, float m, float s) const {
+        if (logp) logp[col] = static_cast<float>(lp);
+        if (exact) exact[col] = lp;
         if (ENTROPY) entropy[col] = h;
         if (stats) {
             stats[col] = m;
             stats[static_cast<size_t>(N) + col] = s;
         }
     }
-    __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f); }
+    __device__ void idle(size_t col) const { write(col, 0.0, 0.f, 0.f, 0.f); }
     template <class T>
     __device__ Grad finish(const T& lead, char*, const Early& e, size_t col, const ColumnSums& c) const {
-        const float lp = static_cast<float>(log_prob(e.x, c));
+        const double lp = log_prob(e.x, c);
         const float h = ENTROPY ? static_cast<float>(entropy_of(c)) : 0.f;
         if (lead.rank == 0) write(col, lp, h, c.m, static_cast<float>(c.s));
         return Grad{};
@@ -42,35 +45,34 @@ struct LogprobHead {
 
 // d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
 // is left, every element is read and written once.  A team of G threads takes 16*G
-// logits of a column.
-constexpr int kBwdBlock = 256, kBwdQuads = 4;
+// logits [begin, begin + len) of a column.
+constexpr int kBwdBlock = 256;
+struct BwdArgs {
+    float* d;
+    const float *g, *x;
+    const int32_t* labels;
+    const float* stats;
+    int K, N;
+    size_t ld, ldd;
+    ExpScale scale;
+};
 template <int G, bool NT>
-__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const float* g, const float* x,
-                                                                const int32_t* labels, const float* stats, int K,
-                                                                int N, int chunks, size_t ld, size_t ldd,
-                                                                ExpScale scale) {
-    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
-    const Team<G> team{static_cast<int>(threadIdx.x % G)};
-    const size_t piece = static_cast<size_t>(blockIdx.x) * kTeams + threadIdx.x / G;
-    const size_t col = kTeams > 1 ? piece : piece / chunks;
-    if (col >= static_cast<size_t>(N)) return;
-    const int begin = kTeams > 1 ? 0 : static_cast<int>(piece % chunks) * kSpan;
-    const int len = K - begin < kSpan ? K - begin : kSpan;
-    const float* p = x + col * ld + begin;
-    float* out = d + col * ldd + begin;
+__device__ __forceinline__ void bwd_span(const BwdArgs& a, const Team<G>& team, size_t col, int begin, int len) {
+    const float* p = a.x + col * a.ld + begin;
+    float* out = a.d + col * a.ldd + begin;
     const Span span = span_of<(G > 4)>(out, len);
     float* const to = out + span.skew;
-    const int label = labels[col];
-    const float up = g[col], m = stats[col], s = stats[static_cast<size_t>(N) + col];
-    const bool live = label_scored(label, K) && s != 0.f && up != 0.f;
+    const int label = a.labels[col];
+    const float up = a.g[col], m = a.stats[col], s = a.stats[static_cast<size_t>(a.N) + col];
+    const bool live = label_scored(label, a.K) && s != 0.f && up != 0.f;
     if (!live) {
         for (int q = team.rank; q < span.quads; q += G) store_quad<NT>(to + 4 * q, Quad(0.f));
         if (team.rank < span.odd) out[span.single(team.rank)] = 0.f;
         return;
     }
-    Quad v[kBwdQuads];
+    Quad v[kGroupQuads];
 #pragma unroll
-    for (int k = 0; k < kBwdQuads; ++k) {
+    for (int k = 0; k < kGroupQuads; ++k) {
         const int q = team.rank + k * G;
         if (q < span.quads) v[k] = load_quad<NT>(p + span.skew + 4 * q);
     }
@@ -79,48 +81,64 @@ __global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(float* d, const 
     Grad f{static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)), 0.f, up, 0.f};
     if (mine) {
         f.x = p[label - begin];
-        if constexpr (kTeams == 1) __syncthreads();   // the gradient may replace the logits
-        else team.sync();
+        team.sync();   // the gradient may replace the logits
     }
-    auto value = [&](float y) { return exp_shifted(y - m, scale) * f.a; };
+    auto value = [&](float y) { return exp_shifted(y - m, a.scale) * f.a; };
 #pragma unroll
-    for (int k = 0; k < kBwdQuads; ++k) {
+    for (int k = 0; k < kGroupQuads; ++k) {
         const int q = team.rank + k * G;
         if (q < span.quads)
             store_quad<NT>(to + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
     if (team.rank < span.odd) out[span.single(team.rank)] = value(last);
-    if (mine) correct_label<false>(team, label - begin, span, m, f, scale, out);
+    if (mine) correct_label<false>(team, label - begin, span, m, f, a.scale, out);
 }
 
-int logprobs(float* logp, float* entropy, float* stats, float* scratch, const float* x, const int32_t* labels, int K,
-             int N, size_t ld) {
+// The sum of the pairs' losses, which the gradient's first workgroup adds up on the way.
+struct PairTotal {
+    float* out;   // null: none
+    const double* losses;
+    int pairs;
+    double scale;
+};
+template <int G, bool NT>
+__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, int chunks, bool backwards) {
+    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kGroupQuads;
+    __shared__ double slots[kBwdBlock / kWave];
+    if (total.out && blockIdx.x == 0) fold_parts<kBwdBlock>(total.out, total.losses, total.pairs, total.scale, slots);
+    const Team<G> team{static_cast<int>(threadIdx.x % G)};
+    const size_t piece = static_cast<size_t>(blockIdx.x) * kTeams + threadIdx.x / G;
+    size_t col = kTeams > 1 ? piece : piece / chunks;
+    if (col >= static_cast<size_t>(a.N)) return;
+    if (backwards) col = static_cast<size_t>(a.N) - 1 - col;
+    const int begin = kTeams > 1 ? 0 : static_cast<int>(piece % chunks) * kSpan;
+    bwd_span<G, NT>(a, team, col, begin, a.K - begin < kSpan ? a.K - begin : kSpan);
+}
+
+int logprobs(float* logp, float* entropy, float* stats, double* exact, float* scratch, const float* x,
+             const int32_t* labels, int K, int N, size_t ld) {
     if (entropy)
-        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N}, TokenSums{},
+        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N, exact}, TokenSums{},
                                    scratch, nullptr, x, K, N, ld, ld);
-    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N}, TokenSums{}, scratch,
+    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N, exact}, TokenSums{}, scratch,
                                nullptr, x, K, N, ld, ld);
 }
 
 template <int G>
-int launch_bwd(float* d, const float* g, const float* x, const int32_t* labels, const float* stats, int K, int N,
-               size_t ld, size_t ldd) {
-    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kBwdQuads;
-    const int chunks = kTeams > 1 ? 1 : (K + kSpan - 1) / kSpan;
-    const size_t blocks = (static_cast<size_t>(N) * chunks + kTeams - 1) / kTeams;
-    const bool nt = streams_past_cache(static_cast<size_t>(K) * N * 2 * sizeof(float));
+int launch_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
+    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kGroupQuads;
+    const int chunks = kTeams > 1 ? 1 : (a.K + kSpan - 1) / kSpan;
+    const size_t blocks = (static_cast<size_t>(a.N) * chunks + kTeams - 1) / kTeams;
+    const bool nt = streams_past_cache(static_cast<size_t>(a.K) * a.N * 2 * sizeof(float));
     auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
-    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(d, g, x, labels, stats, K, N, chunks, ld, ldd,
-                                                                      exp_scale(1.0));
+    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(a, total, chunks, backwards);
     return launch_rc();
 }
-
-int logprobs_bwd(float* d, const float* g, const float* x, const int32_t* labels, const float* stats, int K, int N,
-                 size_t ld, size_t ldd) {
-    if (K <= 64) return launch_bwd<4>(d, g, x, labels, stats, K, N, ld, ldd);
-    if (K <= 256) return launch_bwd<16>(d, g, x, labels, stats, K, N, ld, ldd);
-    if (K <= 1024) return launch_bwd<64>(d, g, x, labels, stats, K, N, ld, ldd);
-    return launch_bwd<256>(d, g, x, labels, stats, K, N, ld, ldd);
+int logprobs_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
+    if (a.K <= 64) return launch_bwd<4>(a, total, backwards);
+    if (a.K <= 256) return launch_bwd<16>(a, total, backwards);
+    if (a.K <= 1024) return launch_bwd<64>(a, total, backwards);
+    return launch_bwd<256>(a, total, backwards);
 }
 
 // ── paired log ratios ────────────────────────────────────────────────────
@@ -134,60 +152,95 @@ constexpr int kPairsPerLaunch = 64;
 struct PairBegins {
     int at[2 * kPairsPerLaunch + 1];
 };
-constexpr int kPairBlock = 256;
-__global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(
-    float* g, float* rewards, double* losses, const float* x, const int32_t* labels, const float* stats,
-    const float* ref, PairBegins begins, int K, int N, size_t ld, int kind, float beta, float smoothing, int average,
-    float scale) {
-    __shared__ double slots[4][kPairBlock / kWave];
-    const Team<kPairBlock> team{static_cast<int>(threadIdx.x)};
-    const int pair = blockIdx.x;
+struct PairArgs {
+    float* g;   // dl/dlogp of every token, or null
+    float* rewards;
+    double* losses;
+    const double* logp;
+    const int32_t* labels;
+    const float *stats, *ref;   // ref may be null
+    PairBegins begins;
+    int K, N, kind, average;
+    float beta, smoothing, scale;
+};
+// One pair by one team; slots: 4*kWaves values in LDS.
+template <class T>
+__device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int pair, double* slots) {
     double reward[2], share[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const int lo = begins.at[2 * pair + k], hi = begins.at[2 * pair + k + 1];
+        const int lo = a.begins.at[2 * pair + k], hi = a.begins.at[2 * pair + k + 1];
         double gain = 0.0, count = 0.0;
-        for (int n = lo + team.rank; n < hi; n += kPairBlock) {
-            const int label = labels[n];
-            const float s = stats[static_cast<size_t>(N) + n];
-            if (!label_scored(label, K) || s == 0.f) continue;
-            const ColumnSums c{stats[n], static_cast<double>(s), 0.0, 0.0};
-            gain += log_prob(x[static_cast<size_t>(n) * ld + label], c) - (ref ? static_cast<double>(ref[n]) : 0.0);
+        for (int n = lo + team.rank; n < hi; n += T::kSize) {
+            if (!label_scored(a.labels[n], a.K) || a.stats[static_cast<size_t>(a.N) + n] == 0.f) continue;
+            gain += a.logp[n] - (a.ref ? static_cast<double>(a.ref[n]) : 0.0);
             count += 1.0;
         }
-        gain = team.reduce(gain, AddOp{}, slots[2 * k]);
-        count = team.reduce(count, AddOp{}, slots[2 * k + 1]);
-        share[k] = average ? (count > 0.0 ? 1.0 / count : 0.0) : 1.0;
-        reward[k] = static_cast<double>(beta) * gain * share[k];
+        gain = team.reduce(gain, AddOp{}, slots + 2 * k * T::kWaves);
+        count = team.reduce(count, AddOp{}, slots + (2 * k + 1) * T::kWaves);
+        share[k] = a.average ? (count > 0.0 ? 1.0 / count : 0.0) : 1.0;
+        reward[k] = static_cast<double>(a.beta) * gain * share[k];
     }
     const double h = reward[0] - reward[1];
     double loss, slope;   // of h; the comparisons are written so that a NaN stays one
-    if (kind == kSigmoid) {
+    if (a.kind == kSigmoid) {
         const double z = exp(-fabs(h)), tail = log1p(z);
         const double down = (h >= 0.0 ? z : 1.0) / (1.0 + z), up = (h >= 0.0 ? 1.0 : z) / (1.0 + z);   // sigma(-h), sigma(h)
-        const double sm = static_cast<double>(smoothing);
+        const double sm = static_cast<double>(a.smoothing);
         loss = (1.0 - sm) * (tail + (h >= 0.0 ? 0.0 : -h)) + sm * (tail + (h >= 0.0 ? h : 0.0));
         slope = -(1.0 - sm) * down + sm * up;
-    } else if (kind == kHinge) {
+    } else if (a.kind == kHinge) {
         loss = h >= 1.0 ? 0.0 : 1.0 - h;
         slope = h >= 1.0 ? 0.0 : (h < 1.0 ? -1.0 : h);
     } else {
-        const double off = (h - 0.5) / static_cast<double>(beta);
+        const double off = (h - 0.5) / static_cast<double>(a.beta);
         loss = off * off;
-        slope = 2.0 * off / static_cast<double>(beta);
+        slope = 2.0 * off / static_cast<double>(a.beta);
     }
     if (team.rank == 0) {
-        rewards[2 * pair] = static_cast<float>(reward[0]);
-        rewards[2 * pair + 1] = static_cast<float>(reward[1]);
-        losses[pair] = loss;
+        a.rewards[2 * pair] = static_cast<float>(reward[0]);
+        a.rewards[2 * pair + 1] = static_cast<float>(reward[1]);
+        a.losses[pair] = loss;
     }
-    if (!g) return;
+    if (!a.g) return;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const double v = (k ? -slope : slope) * share[k] * static_cast<double>(beta) * static_cast<double>(scale);
-        for (int n = begins.at[2 * pair + k] + team.rank; n < begins.at[2 * pair + k + 1]; n += kPairBlock)
-            g[n] = static_cast<float>(v);
+        const double v = (k ? -slope : slope) * share[k] * static_cast<double>(a.beta) * static_cast<double>(a.scale);
+        for (int n = a.begins.at[2 * pair + k] + team.rank; n < a.begins.at[2 * pair + k + 1]; n += T::kSize)
+            a.g[n] = static_cast<float>(v);
     }
+}
+constexpr int kPairBlock = 256;
+__global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(PairArgs a) {
+    __shared__ double slots[4 * kPairBlock / kWave];
+    take_pair(a, Team<kPairBlock>{static_cast<int>(threadIdx.x)}, blockIdx.x, slots);
+}
+
+// Short sequences over few classes: all three steps and the sum in one workgroup, since the
+// work is less than the launches (2 pairs, 90 tokens x 256: 16 -> 7 us).
+constexpr int kSmallBlock = 1024, kSmallRounds = 4;
+template <int G>
+__global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHead<false> head, PairArgs pairs, BwdArgs bwd,
+                                                                       PairTotal total) {
+    constexpr int kTeams = kSmallBlock / G;
+    __shared__ ColumnShared<G> shared;
+    __shared__ double slots[kSmallBlock / kWave];
+    const Team<G> team{static_cast<int>(threadIdx.x % G)};
+    for (int n = threadIdx.x / G; n < bwd.N; n += kTeams)
+        token_column<LogprobHead<false>, G, kGroupQuads, false, false>(head, team, shared, nullptr, n, nullptr,
+                                                                       bwd.x + n * bwd.ld, bwd.K);
+    __syncthreads();
+    const Team<kWave> wave{static_cast<int>(threadIdx.x % kWave)};
+    for (int p = threadIdx.x / kWave; p < total.pairs; p += kSmallBlock / kWave) take_pair(pairs, wave, p, nullptr);
+    __syncthreads();
+    if (bwd.d)
+        for (int n = threadIdx.x / G; n < bwd.N; n += kTeams) bwd_span<G, false>(bwd, team, n, 0, bwd.K);
+    fold_parts<kSmallBlock>(total.out, total.losses, total.pairs, total.scale, slots);
+}
+template <int G>
+int launch_small(const LogprobHead<false>& head, const PairArgs& pairs, const BwdArgs& bwd, const PairTotal& total) {
+    preference_small_kernel<G><<<1, kSmallBlock, 0, stream()>>>(head, pairs, bwd, total);
+    return launch_rc();
 }
 
 }  // namespace
@@ -204,14 +257,15 @@ JZ_API int jzhip_token_logprobs(float* logp, float* entropy, float* stats, float
                                 const int32_t* labels, int K, int N, int ld) {
     if (!token_args_ok(logits, nullptr, scratch, K, N, ld, ld) || !labels || !scratch || (!logp && !entropy && !stats))
         return -1;
-    return logprobs(logp, entropy, stats, scratch, logits, labels, K, N, static_cast<size_t>(ld));
+    return logprobs(logp, entropy, stats, nullptr, scratch, logits, labels, K, N, static_cast<size_t>(ld));
 }
 
 JZ_API int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const float* logits, const int32_t* labels,
                                     const float* stats, int K, int N, int ld, int ldd) {
     if (!token_args_ok(logits, dlogits, nullptr, K, N, ld, ldd) || !dlogits || !dlogp || !labels || !stats) return -1;
-    return logprobs_bwd(dlogits, dlogp, logits, labels, stats, K, N, static_cast<size_t>(ld),
-                        static_cast<size_t>(ldd));
+    return logprobs_bwd(BwdArgs{dlogits, dlogp, logits, labels, stats, K, N, static_cast<size_t>(ld),
+                                static_cast<size_t>(ldd), exp_scale(1.0)},
+                        PairTotal{}, false);
 }
 
 JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* stats, float* dlogits,
@@ -228,20 +282,37 @@ JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, f
     const int N = seq_begin[2 * pairs];
     if (!token_args_ok(logits, dlogits, scratch, K, N, ld, ldd)) return -1;
     double* losses = reinterpret_cast<double*>(scratch);
-    float* g = scratch + kScratchFixed;
+    double* exact = reinterpret_cast<double*>(scratch + kScratchFixed);
+    float* g = dlogits ? scratch + kScratchFixed + 2 * static_cast<size_t>(N) : nullptr;
     const size_t ldx = static_cast<size_t>(ld);
-    int rc = logprobs(logp, nullptr, stats, scratch, logits, labels, K, N, ldx);
+    const BwdArgs bwd{dlogits, g, logits, labels, stats, K, N, ldx, static_cast<size_t>(ldd), exp_scale(1.0)};
+    const PairTotal total{loss_out, losses, pairs, static_cast<double>(scale)};
+    PairArgs args{g, rewards, losses, exact, labels, stats, ref_logp, {}, K, N, kind, average, beta, smoothing, scale};
+    auto begins = [&](int at, int n) {
+        for (int i = 0; i <= 2 * n; ++i) args.begins.at[i] = seq_begin[2 * at + i];
+        args.rewards = rewards + 2 * at;
+        args.losses = losses + at;
+    };
+    if (K <= 1024 && pairs <= kPairsPerLaunch) {
+        const int lanes = K <= 64 ? 4 : K <= 256 ? 16 : 64;
+        if (N <= kSmallRounds * kSmallBlock / lanes) {
+            begins(0, pairs);
+            const LogprobHead<false> head{exp_scale(1.0), labels, logp, nullptr, stats, N, exact};
+            if (lanes == 4) return launch_small<4>(head, args, bwd, total);
+            if (lanes == 16) return launch_small<16>(head, args, bwd, total);
+            return launch_small<64>(head, args, bwd, total);
+        }
+    }
+    int rc = logprobs(logp, nullptr, stats, exact, scratch, logits, labels, K, N, ldx);
     for (int at = 0; rc == 0 && at < pairs; at += kPairsPerLaunch) {
         const int n = pairs - at < kPairsPerLaunch ? pairs - at : kPairsPerLaunch;
-        PairBegins begins = {};
-        for (int i = 0; i <= 2 * n; ++i) begins.at[i] = seq_begin[2 * at + i];
-        preference_pair_kernel<<<n, kPairBlock, 0, stream()>>>(dlogits ? g : nullptr, rewards + 2 * at, losses + at,
-                                                               logits, labels, stats, ref_logp, begins, K, N, ldx,
-                                                               kind, beta, smoothing, average, scale);
+        begins(at, n);
+        preference_pair_kernel<<<n, kPairBlock, 0, stream()>>>(args);
         rc = launch_rc();
     }
-    if (rc == 0 && dlogits) rc = logprobs_bwd(dlogits, g, logits, labels, stats, K, N, ldx, static_cast<size_t>(ldd));
     if (rc) return rc;
+    // the last columns read are the first ones read again: they are in the cache
+    if (dlogits) return logprobs_bwd(bwd, total, true);
     token_fold_kernel<double><<<1, kFoldBlock, 0, stream()>>>(loss_out, losses, pairs, 0, static_cast<double>(scale));
     return launch_rc();
 }

@@ -10,10 +10,10 @@
 // What bounds all of them is memory: 8 bytes per logit against about a dozen vector
 // instructions.
 //
-// Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.
-// Losses over many tokens cancel (the reward of an answer is a sum of small differences
-// of log-probabilities), so a bias of a few 1e-8 per token would show in them: sums in
-// fp32 alone made rewards ten times less exact.  What happens once per column (log s,
+// Accuracy: a thread adds sixteen exponentials in fp32, those that are 1 apart, and everything
+// further in 64 bits.  Losses over many tokens cancel (the reward of an answer is a sum of
+// small differences of log-probabilities), so an error of a few 1e-8 per token shows in
+// them: sums in fp32 alone made rewards ten times less exact.  What happens once per column (log s,
 // ratios, divergences) is done in 64 bits too.
 #pragma once
 
@@ -244,25 +244,29 @@ __device__ __forceinline__ float quad_max(const Quad& v) { return fmaxf(fmaxf(v.
 // only a factor exp(m_group - m) once that is known.
 constexpr int kGroupQuads = 4;
 struct Group {
-    float m, s, et, rest;
+    float m, s, ones, et, rest;   // s: of the exponentials below 1, ones: how many are 1
 };
 // x: the group's logits; without the entropy they become e_i relative to the group.  known(k): the
 // teacher's entries among quad k.
 template <class Head, class Known>
 __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpScale& scale, Known known) {
-    Group g{-INFINITY, 0.f, 0.f, 0.f};
+    Group g{-INFINITY, 0.f, 0.f, 0.f, 0.f};
     float top[kGroupQuads];
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) top[k] = quad_max(x[k]);
     g.m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     const float shift = g.m == -INFINITY ? 0.f : g.m;   // nothing but -inf: sums of 0; a NaN still shows
-    float s[kGroupQuads], et[kGroupQuads], rest[kGroupQuads];
+    float s[kGroupQuads], all[kGroupQuads], et[kGroupQuads], rest[kGroupQuads];
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) {
         const float t0 = x[k].x - shift, t1 = x[k].y - shift, t2 = x[k].z - shift, t3 = x[k].w - shift;
         const float e0 = exp_shifted(t0, scale), e1 = exp_shifted(t1, scale);
         const float e2 = exp_shifted(t2, scale), e3 = exp_shifted(t3, scale);
-        s[k] = (e0 + e1) + (e2 + e3);
+        // Where one logit stands out, what the others add to its 1 is what log s is made of, and fp32 would
+        // round it at 2^-24: the ones are counted apart (an exponential is its own fraction otherwise).
+        all[k] = (e0 + e1) + (e2 + e3);
+        s[k] = (__builtin_amdgcn_fractf(e0) + __builtin_amdgcn_fractf(e1)) +
+               (__builtin_amdgcn_fractf(e2) + __builtin_amdgcn_fractf(e3));
         if constexpr (Head::kEntropy)
             et[k] = (e0 * fmaxf(t0, -200.f) + e1 * fmaxf(t1, -200.f)) + (e2 * fmaxf(t2, -200.f) + e3 * fmaxf(t3, -200.f));
         else
@@ -273,6 +277,7 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
         }
     }
     g.s = (s[0] + s[1]) + (s[2] + s[3]);
+    g.ones = rintf(((all[0] + all[1]) + (all[2] + all[3])) - g.s);
     if constexpr (Head::kEntropy) g.et = (et[0] + et[1]) + (et[2] + et[3]);
     if constexpr (Head::kRest) g.rest = (rest[0] + rest[1]) + (rest[2] + rest[3]);
     return g;
@@ -291,7 +296,7 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
 }
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
-    ColumnSums more{g.m, static_cast<double>(g.s), static_cast<double>(g.et), static_cast<double>(g.rest)};
+    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s), static_cast<double>(g.et), static_cast<double>(g.rest)};
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
     scale_sums<Head>(more, m, scale);
@@ -303,7 +308,7 @@ __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const E
 template <class Head>
 __device__ __forceinline__ Group take_one(float x, bool known) {
     const float e = x == -INFINITY ? 0.f : x - x + 1.f;   // exp of its shift from itself; a NaN or +inf shows
-    return Group{x, e, 0.f, known ? 0.f : e};
+    return Group{x, 0.f, e, 0.f, known ? 0.f : e};
 }
 
 // The compiler would interleave the independent work of an unrolled loop and spill what it
@@ -786,7 +791,7 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                          size_t ldd) {
-    if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
+    if (!head.read_again() && streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
         return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
     return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }

@@ -26,6 +26,7 @@ struct PolicyHead {
     int N;
 
     __host__ __device__ size_t team_bytes(int) const { return 0; }
+    bool read_again() const { return false; }
     __device__ bool live(size_t col, int K) const {
         return label_scored(labels[col], K) && !(weight && weight[col] == 0.f);
     }
