@@ -180,9 +180,9 @@ struct DistillHead {
         return f;
     }
     template <class T>
-    __device__ void correct(const T& team, char* own, size_t, float m, const Grad& f, float* out, const Span&) const {
+    __device__ void correct(const T& lead, char* own, size_t, float m, const Grad& f, float* out) const {
         const Entries e(own, top);
-        for (int j = team.rank; j < top; j += T::kLanes)
+        for (int j = lead.rank; j < top; j += T::kSize)
             if (e.id[j] >= 0) out[e.id[j]] = entry_gradient(e, j, m, f);
     }
     // The entries among the logits [begin, begin + len), whose gradients `picked` holds.

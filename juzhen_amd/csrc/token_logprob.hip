@@ -40,12 +40,14 @@ struct LogprobHead {
         return Grad{};
     }
     template <class T>
-    __device__ void correct(const T&, char*, size_t, float, const Grad&, float*, const Span&) const {}
+    __device__ void correct(const T&, char*, size_t, float, const Grad&, float*) const {}
 };
 
 // d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
-// is left, every element is read and written once.  A team of G threads takes 16*G
-// logits [begin, begin + len) of a column.
+// is left, every element is read and written once.  A team takes NV*G quads of a column,
+// from quad `base` on; the one that begins at 0 its single logits as well.  Long columns are
+// cut into workgroups of one quad per thread: many small workgroups keep the accesses in
+// flight closest together (32000 x 4194: 1 quad 166 us, 2 180, 4 193, 8 194).
 constexpr int kBwdBlock = 256;
 struct BwdArgs {
     float* d;
@@ -56,42 +58,51 @@ struct BwdArgs {
     size_t ld, ldd;
     ExpScale scale;
 };
-template <int G, bool NT>
-__device__ __forceinline__ void bwd_span(const BwdArgs& a, const Team<G>& team, size_t col, int begin, int len) {
-    const float* p = a.x + col * a.ld + begin;
-    float* out = a.d + col * a.ldd + begin;
-    const Span span = span_of<(G > 4)>(out, len);
-    float* const to = out + span.skew;
+template <int G, int NV, bool NT>
+__device__ __forceinline__ void bwd_span(const BwdArgs& a, const Team<G>& team, size_t col, int base) {
+    const float* p = a.x + col * a.ld;
+    float* out = a.d + col * a.ldd;
+    const Span span = span_of<(G > 4)>(out, a.K);
+    const int singles = base == 0 ? span.odd : 0;
     const int label = a.labels[col];
     const float up = a.g[col], m = a.stats[col], s = a.stats[static_cast<size_t>(a.N) + col];
     const bool live = label_scored(label, a.K) && s != 0.f && up != 0.f;
     if (!live) {
-        for (int q = team.rank; q < span.quads; q += G) store_quad<NT>(to + 4 * q, Quad(0.f));
-        if (team.rank < span.odd) out[span.single(team.rank)] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int q = base + team.rank + k * G;
+            if (q < span.quads) store_quad<NT>(out + span.skew + 4 * static_cast<size_t>(q), Quad(0.f));
+        }
+        if (team.rank < singles) out[span.single(team.rank)] = 0.f;
         return;
     }
-    Quad v[kGroupQuads];
+    Quad v[NV];
 #pragma unroll
-    for (int k = 0; k < kGroupQuads; ++k) {
-        const int q = team.rank + k * G;
-        if (q < span.quads) v[k] = load_quad<NT>(p + span.skew + 4 * q);
+    for (int k = 0; k < NV; ++k) {
+        const int q = base + team.rank + k * G;
+        if (q < span.quads) v[k] = load_quad<NT>(p + span.skew + 4 * static_cast<size_t>(q));
     }
-    const float last = team.rank < span.odd ? p[span.single(team.rank)] : 0.f;
-    const bool mine = label >= begin && label < begin + len;
+    const float last = team.rank < singles ? p[span.single(team.rank)] : 0.f;
+    const int quad = (label - span.skew) / 4;
+    const bool mine = label < span.skew || quad >= span.quads ? base == 0 : quad >= base && quad < base + NV * G;
     Grad f{static_cast<float>(-static_cast<double>(up) / static_cast<double>(s)), 0.f, up, 0.f};
     if (mine) {
-        f.x = p[label - begin];
+        f.x = p[label];
         team.sync();   // the gradient may replace the logits
     }
     auto value = [&](float y) { return exp_shifted(y - m, a.scale) * f.a; };
 #pragma unroll
-    for (int k = 0; k < kGroupQuads; ++k) {
-        const int q = team.rank + k * G;
+    for (int k = 0; k < NV; ++k) {
+        const int q = base + team.rank + k * G;
         if (q < span.quads)
-            store_quad<NT>(to + 4 * q, Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
+            store_quad<NT>(out + span.skew + 4 * static_cast<size_t>(q),
+                           Quad{value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w)});
     }
-    if (team.rank < span.odd) out[span.single(team.rank)] = value(last);
-    if (mine) correct_label<false>(team, label - begin, span, m, f, a.scale, out);
+    if (team.rank < singles) out[span.single(team.rank)] = value(last);
+    if (mine) {
+        team.sync();
+        if (team.rank == 0) correct_label<false>(label, m, f, a.scale, out);
+    }
 }
 
 // The sum of the pairs' losses, which the gradient's first workgroup adds up on the way.
@@ -101,18 +112,18 @@ struct PairTotal {
     int pairs;
     double scale;
 };
+// G < 256: a column per team; 256: `chunks` workgroups per column
 template <int G, bool NT>
-__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, int chunks, bool backwards) {
-    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kGroupQuads;
+__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, FastDiv chunks, bool backwards) {
+    constexpr int kTeams = kBwdBlock / G;
     __shared__ double slots[kBwdBlock / kWave];
     if (total.out && blockIdx.x == 0) fold_parts<kBwdBlock>(total.out, total.losses, total.pairs, total.scale, slots);
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
-    const size_t piece = static_cast<size_t>(blockIdx.x) * kTeams + threadIdx.x / G;
-    size_t col = kTeams > 1 ? piece : piece / chunks;
-    if (col >= static_cast<size_t>(a.N)) return;
-    if (backwards) col = static_cast<size_t>(a.N) - 1 - col;
-    const int begin = kTeams > 1 ? 0 : static_cast<int>(piece % chunks) * kSpan;
-    bwd_span<G, NT>(a, team, col, begin, a.K - begin < kSpan ? a.K - begin : kSpan);
+    int col = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
+    if (kTeams > 1 && col >= a.N) return;
+    const int base = kTeams > 1 ? 0 : static_cast<int>(blockIdx.x - col * chunks.d) * G;
+    if (backwards) col = a.N - 1 - col;
+    bwd_span<G, (G < kBwdBlock ? kGroupQuads : 1), NT>(a, team, col, base);
 }
 
 int logprobs(float* logp, float* entropy, float* stats, double* exact, float* scratch, const float* x,
@@ -126,12 +137,13 @@ int logprobs(float* logp, float* entropy, float* stats, double* exact, float* sc
 
 template <int G>
 int launch_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
-    constexpr int kTeams = kBwdBlock / G, kSpan = 4 * G * kGroupQuads;
-    const int chunks = kTeams > 1 ? 1 : (a.K + kSpan - 1) / kSpan;
+    constexpr int kTeams = kBwdBlock / G;
+    const int chunks = kTeams > 1 ? 1 : (a.K / 4 + G - 1) / G;
     const size_t blocks = (static_cast<size_t>(a.N) * chunks + kTeams - 1) / kTeams;
+    if (blocks > 0x7fffffffull) return -1;
     const bool nt = streams_past_cache(static_cast<size_t>(a.K) * a.N * 2 * sizeof(float));
     auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
-    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(a, total, chunks, backwards);
+    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(a, total, make_fastdiv(chunks), backwards);
     return launch_rc();
 }
 int logprobs_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHe
     for (int p = threadIdx.x / kWave; p < total.pairs; p += kSmallBlock / kWave) take_pair(pairs, wave, p, nullptr);
     __syncthreads();
     if (bwd.d)
-        for (int n = threadIdx.x / G; n < bwd.N; n += kTeams) bwd_span<G, false>(bwd, team, n, 0, bwd.K);
+        for (int n = threadIdx.x / G; n < bwd.N; n += kTeams) bwd_span<G, kGroupQuads, false>(bwd, team, n, 0);
     fold_parts<kSmallBlock>(total.out, total.losses, total.pairs, total.scale, slots);
 }
 template <int G>

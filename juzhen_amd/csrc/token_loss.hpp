@@ -37,10 +37,13 @@ inline ExpScale exp_scale(double temperature) {
     return r;
 }
 
-// exp(d/T) for d <= 0: the hardware's 2^u (0.7 ulp, mean error 3e-9; an exact 0 below
+// exp(d/T) for d <= 0: the hardware's 2^u (0.7 ulp, mean error kExpShort; an exact 0 below
 // 2^-126) of u = d*log2(e)/T rounded once.  The low part of the constant is what keeps
 // the result without bias (-1.3e-8 * u otherwise); it is positive, so that d = -inf
 // gives -inf - inf and 0.  A NaN stays one.
+// What the hardware's 2^u falls short of on average (over u in [-1, 0], [-8, 0] and [-40, 0] alike,
+// but for the exact 1 at 0): sums put it back.
+constexpr double kExpShort = 3.4e-9;
 __device__ __forceinline__ float exp_shifted(float d, const ExpScale& c) {
     return __builtin_amdgcn_exp2f(fmaf(d, c.hi, d * c.lo));
 }
@@ -205,11 +208,6 @@ typedef float Quad __attribute__((ext_vector_type(4), aligned(4)));
 struct Span {
     int skew, quads, odd;
     __device__ __forceinline__ int single(int r) const { return r < skew ? r : 4 * quads + r; }
-    // the thread of a team of G that has element i
-    __device__ __forceinline__ int owner(int i, int G) const {
-        const int q = i < skew ? quads : (i - skew) / 4;
-        return q < quads ? q % G : i < skew ? i : i - 4 * quads;
-    }
 };
 // ALIGN: an odd leading dimension costs a wave's 1 KB access a ninth cache line otherwise.
 template <bool ALIGN>
@@ -288,7 +286,7 @@ template <class Head>
 __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScale& scale) {
     if (m == -INFINITY) return;
     const float t = c.m - m;
-    const double f = static_cast<double>(exp_shifted(t, scale));
+    const double f = t == 0.f ? 1.0 : static_cast<double>(exp_shifted(t, scale)) * (1.0 + kExpShort);
     if constexpr (Head::kEntropy) c.et = (c.et + c.s * static_cast<double>(fmaxf(t, -200.f))) * f;
     if constexpr (Head::kRest) c.rest *= f;
     c.s *= f;
@@ -296,7 +294,8 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
 }
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
-    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s), static_cast<double>(g.et), static_cast<double>(g.rest)};
+    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s) * (1.0 + kExpShort),
+                    static_cast<double>(g.et), static_cast<double>(g.rest)};
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
     scale_sums<Head>(more, m, scale);
@@ -318,15 +317,28 @@ __device__ __forceinline__ void in_order() {
     if constexpr (NV > kGroupQuads) __builtin_amdgcn_sched_barrier(0);
 }
 
-// The label's element: the thread that wrote it writes it again.
-template <bool LINEAR, class T>
-__device__ __forceinline__ void correct_label(const T& team, int label, const Span& span, float m, const Grad& f,
-                                              const ExpScale& scale, float* out) {
-    if (team.rank == span.owner(label, T::kSize)) {
-        const float t = f.x - m;
-        out[label] = grad_value<LINEAR>(t, exp_shifted(t, scale), f.a, f.b) + f.g;
-    }
+// The label's element, behind the sweep that wrote it as any other: after a team.sync(), by one thread.
+template <bool LINEAR>
+__device__ __forceinline__ void correct_label(int label, float m, const Grad& f, const ExpScale& scale, float* out) {
+    const float t = f.x - m;
+    out[label] = grad_value<LINEAR>(t, exp_shifted(t, scale), f.a, f.b) + f.g;
 }
+
+// Where the quads of a tile lie: up to NV per thread from quad `base` on, those of a wave one
+// stretch of memory (a wave that strides by the workgroup's width instead: 5 % slower, 193
+// against 182 us for one read and one write of 512 MB each).
+template <int G, int NV>
+struct Tile {
+    int first, count;   // of this thread: quads first + k*kLanes, k < count
+    static constexpr int kLanes = Team<G>::kLanes;
+    __device__ __forceinline__ Tile(int rank, int base, int quads) {
+        const int n = (quads - base + G - 1) / G;
+        count = n < NV ? n : NV;
+        first = base + rank / kLanes * kLanes * count + rank % kLanes;
+    }
+    __device__ __forceinline__ int at(int k) const { return first + k * kLanes; }
+    __device__ __forceinline__ bool has(int k, int quads) const { return k < count && at(k) < quads; }
+};
 
 template <int G>
 struct ColumnShared {
@@ -348,6 +360,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     constexpr bool kKeepMax = Head::kWrites && !Head::kEntropy;   // the kept exponentials are relative to it
     const Span span = span_of<(G > 4)>(p, K);   // (by the logits: values are the same bits with and without a gradient)
     const float* const body = p + span.skew;
+    const Tile<G, NV> mine(team.rank, 0, span.quads);
     bool live = head.live(col, K);
     Quad v[kGroups][kGroupQuads];
     float group_max[kGroups];
@@ -356,9 +369,9 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     typename Head::Early early{};
     if (live) {
         const unsigned* bits = nullptr;
-        auto take = [&](Quad (&x)[kGroupQuads], int first) {   // quads first + rank + k*G
+        auto take = [&](Quad (&x)[kGroupQuads], const Tile<G, NV>& tile, int first) {
             const Group g = take_group<Head>(x, head.scale, [&](int k) {
-                const int q = first + team.rank + k * G;
+                const int q = tile.at(first + k);
                 return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));   // (nothing counts behind the column)
             });
             add_group<Head>(c, g, head.scale);
@@ -389,26 +402,25 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         }
         if constexpr (STREAM) {
             for (int base = kTile; base < span.quads; base += kTile) {
+                const Tile<G, NV> tile(team.rank, base, span.quads);
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const int q = base + team.rank + k * G;
                     Quad& x = v[k / kGroupQuads][k % kGroupQuads];
                     x = Quad(-INFINITY);
-                    if (q < span.quads) x = load_quad<NT && !Head::kWrites>(body + 4 * static_cast<size_t>(q));
+                    if (tile.has(k, span.quads)) x = load_quad<NT && !Head::kWrites>(body + 4 * static_cast<size_t>(tile.at(k)));
                 }
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
-                    take(v[i], base + i * kGroupQuads * G);
+                    take(v[i], tile, i * kGroupQuads);
                     in_order<NV>();
                 }
             }
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int q = team.rank + k * G;
             Quad& x = v[k / kGroupQuads][k % kGroupQuads];
             x = Quad(-INFINITY);
-            if (q < span.quads) x = load_quad<NT>(body + 4 * static_cast<size_t>(q));
+            if (mine.has(k, span.quads)) x = load_quad<NT>(body + 4 * static_cast<size_t>(mine.at(k)));
         }
         if (team.rank < span.odd) last = p[span.single(team.rank)];
         if constexpr (Head::kTeacher && !kTeacherFirst) teach();
@@ -418,7 +430,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         }
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) {
-            const float m = take(v[i], i * kGroupQuads * G);
+            const float m = take(v[i], mine, i * kGroupQuads);
             if constexpr (kKeepMax) group_max[i] = m;
             in_order<NV>();
         }
@@ -472,13 +484,12 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         if constexpr (kKeepMax) scale = (c.m == -INFINITY ? 1.f : exp_shifted(group_max[i] - c.m, head.scale)) * f.a;
 #pragma unroll
         for (int k = 0; k < kGroupQuads; ++k) {
-            const int q = team.rank + (i * kGroupQuads + k) * G;
             const Quad x = v[i][k];
-            if (q >= span.quads) continue;
+            if (!mine.has(i * kGroupQuads + k, span.quads)) continue;
             Quad r;
             if constexpr (Head::kEntropy) r = Quad{value(x.x), value(x.y), value(x.z), value(x.w)};   // x: logits
             else r = Quad{x.x * scale, x.y * scale, x.z * scale, x.w * scale};
-            store_quad<NT>(to + 4 * static_cast<size_t>(q), r);
+            store_quad<NT>(to + 4 * static_cast<size_t>(mine.at(i * kGroupQuads + k)), r);
         }
         in_order<NV>();
     }
@@ -486,23 +497,22 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     if constexpr (STREAM) {
         constexpr int kQuads = 8, kStep = kQuads * G;
         for (int base = (span.quads - 1) / kStep * kStep; base >= kTile; base -= kStep) {
+            const Tile<G, kQuads> tile(team.rank, base, span.quads);
             Quad x[kQuads];
 #pragma unroll
             for (int k = 0; k < kQuads; ++k) {
-                const int q = base + team.rank + k * G;
                 x[k] = Quad(0.f);
-                if (q < span.quads) x[k] = load_quad<NT>(body + 4 * static_cast<size_t>(q));
+                if (tile.has(k, span.quads)) x[k] = load_quad<NT>(body + 4 * static_cast<size_t>(tile.at(k)));
             }
 #pragma unroll
             for (int k = 0; k < kQuads; ++k) {
-                const int q = base + team.rank + k * G;
                 const Quad r{value(x[k].x), value(x[k].y), value(x[k].z), value(x[k].w)};
-                if (q < span.quads) store_quad<NT>(to + 4 * static_cast<size_t>(q), r);
+                if (tile.has(k, span.quads)) store_quad<NT>(to + 4 * static_cast<size_t>(tile.at(k)), r);
             }
         }
     }
-    if constexpr (Head::kTeacher) team.sync();   // behind the sweep that wrote these elements as any other
-    if (!Head::kTeacher || team.leads()) head.correct(team, own, col, c.m, f, out, span);
+    team.sync();   // behind the sweep that wrote these elements as any other
+    if (team.leads()) head.correct(team.lead(), own, col, c.m, f, out);
 }
 
 // out[k] = scale * sum_i part[k*stride + i] by a workgroup of BLOCK threads, in 64 bits in a fixed order.
@@ -722,10 +732,9 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, Tok
     }
     if (rank < span.odd) out[span.single(rank)] = value(last);
     const int label = r.label - begin;
-    if (label >= 0 && label < len)
-        correct_label<Head::kEntropy>(Team<kChunkBlock>{rank}, label, span, r.m, r.f, head.scale, out);
+    __syncthreads();   // behind the sweep that wrote these elements as any other
+    if (rank == 0 && label >= 0 && label < len) correct_label<Head::kEntropy>(label, r.m, r.f, head.scale, out);
     if constexpr (Head::kTeacher) {
-        __syncthreads();   // behind the sweep that wrote these elements as any other
         head.correct_chunk(Team<kChunkBlock>{rank}, dynamic, col, begin, len, out);
     }
 }

@@ -78,8 +78,8 @@ struct PolicyHead {
         return Grad{static_cast<float>(a * inv), static_cast<float>(b * inv), static_cast<float>(g * w), e.x};
     }
     template <class T>
-    __device__ void correct(const T& team, char*, size_t col, float m, const Grad& f, float* out, const Span& span) const {
-        correct_label<ENTROPY>(team, labels[col], span, m, f, scale, out);
+    __device__ void correct(const T& lead, char*, size_t col, float m, const Grad& f, float* out) const {
+        if (lead.rank == 0) correct_label<ENTROPY>(labels[col], m, f, scale, out);
     }
 };
 
