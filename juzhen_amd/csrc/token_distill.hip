@@ -29,7 +29,7 @@ struct Entries {
 
 template <bool REST>
 struct DistillHead {
-    static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true;
+    static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true, kExact = false;
     struct Early {
         float w;
         double Q;   // sum of the q_j, from the prologue
@@ -59,7 +59,6 @@ struct DistillHead {
             if (at >= begin && at < begin + len) atomicOr(&all[(at - begin) >> 5], 1u << ((at - begin) & 31));
         }
     }
-    bool read_again() const { return false; }
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
     __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, 0.0}; }

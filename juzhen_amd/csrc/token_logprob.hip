@@ -5,9 +5,10 @@
 namespace jz {
 namespace {
 
-template <bool ENTROPY>
+// EXACT: log p in 64 bits as well, for a loss over many tokens.
+template <bool ENTROPY, bool EXACT>
 struct LogprobHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false, kExact = EXACT;
     struct Early {
         float x;   // the label's logit
     };
@@ -15,16 +16,15 @@ struct LogprobHead {
     const int32_t* labels;
     float *logp, *entropy, *stats;   // each may be null
     int N;
-    double* exact;                   // log p once more for a loss over many tokens, or null
+    double* exact;                   // EXACT
 
     __host__ __device__ size_t team_bytes(int) const { return 0; }
-    bool read_again() const { return exact != nullptr; }   // the gradient's sweep follows: leave the caches be
     __device__ bool live(size_t col, int K) const { return label_scored(labels[col], K); }
     __device__ int label(size_t col) const { return labels[col]; }
     __device__ Early early(size_t col, const float* x) const { return Early{x[labels[col]]}; }
     __device__ void write(size_t col, double lp, float h, float m, float s) const {
         if (logp) logp[col] = static_cast<float>(lp);
-        if (exact) exact[col] = lp;
+        if (EXACT) exact[col] = lp;
         if (ENTROPY) entropy[col] = h;
         if (stats) {
             stats[col] = m;
@@ -46,9 +46,10 @@ struct LogprobHead {
 // d_i = g*(delta_i - e_i/s) from the maximum and the sum of the forward call: no reduction
 // is left, every element is read and written once.  A team takes NV*G quads of a column,
 // from quad `base` on; the one that begins at 0 its single logits as well.  Long columns are
-// cut into workgroups of one quad per thread: many small workgroups keep the accesses in
-// flight closest together (32000 x 4194: 1 quad 166 us, 2 180, 4 193, 8 194).
-constexpr int kBwdBlock = 256;
+// cut into workgroups of 512 threads with one quad each, which keeps the accesses in flight
+// closest together (32000 x 4194, a quarter of the tokens unscored: 151 us, 2 quads 173; 256
+// threads with 1, 2, 4 quads 149, 158, 176, but 163 to 151 at 50001 x 2684).
+constexpr int kBwdBlock = 256, kBwdLong = 512;
 struct BwdArgs {
     float* d;
     const float *g, *x;
@@ -112,45 +113,44 @@ struct PairTotal {
     int pairs;
     double scale;
 };
-// G < 256: a column per team; 256: `chunks` workgroups per column
+// G <= 64: a column per team; else `chunks` workgroups per column
 template <int G, bool NT>
-__global__ __launch_bounds__(kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, FastDiv chunks, bool backwards) {
-    constexpr int kTeams = kBwdBlock / G;
-    __shared__ double slots[kBwdBlock / kWave];
-    if (total.out && blockIdx.x == 0) fold_parts<kBwdBlock>(total.out, total.losses, total.pairs, total.scale, slots);
+__global__ __launch_bounds__(G > kWave ? G : kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, FastDiv chunks,
+                                                                                bool backwards) {
+    constexpr int kBlock = G > kWave ? G : kBwdBlock, kTeams = kBlock / G;
+    __shared__ double slots[kBlock / kWave];
+    if (total.out && blockIdx.x == 0) fold_parts<kBlock>(total.out, total.losses, total.pairs, total.scale, slots);
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
     int col = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
     if (kTeams > 1 && col >= a.N) return;
     const int base = kTeams > 1 ? 0 : static_cast<int>(blockIdx.x - col * chunks.d) * G;
     if (backwards) col = a.N - 1 - col;
-    bwd_span<G, (G < kBwdBlock ? kGroupQuads : 1), NT>(a, team, col, base);
+    bwd_span<G, (kTeams > 1 ? kGroupQuads : 1), NT>(a, team, col, base);
 }
 
+template <bool ENTROPY, bool EXACT>
 int logprobs(float* logp, float* entropy, float* stats, double* exact, float* scratch, const float* x,
              const int32_t* labels, int K, int N, size_t ld) {
-    if (entropy)
-        return launch_token_kernel(LogprobHead<true>{exp_scale(1.0), labels, logp, entropy, stats, N, exact}, TokenSums{},
-                                   scratch, nullptr, x, K, N, ld, ld);
-    return launch_token_kernel(LogprobHead<false>{exp_scale(1.0), labels, logp, nullptr, stats, N, exact}, TokenSums{}, scratch,
-                               nullptr, x, K, N, ld, ld);
+    return launch_token_kernel(LogprobHead<ENTROPY, EXACT>{exp_scale(1.0), labels, logp, entropy, stats, N, exact},
+                               TokenSums{}, scratch, nullptr, x, K, N, ld, ld);
 }
 
 template <int G>
 int launch_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
-    constexpr int kTeams = kBwdBlock / G;
+    constexpr int kBlock = G > kWave ? G : kBwdBlock, kTeams = kBlock / G;
     const int chunks = kTeams > 1 ? 1 : (a.K / 4 + G - 1) / G;
     const size_t blocks = (static_cast<size_t>(a.N) * chunks + kTeams - 1) / kTeams;
     if (blocks > 0x7fffffffull) return -1;
     const bool nt = streams_past_cache(static_cast<size_t>(a.K) * a.N * 2 * sizeof(float));
     auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
-    kernel<<<static_cast<unsigned>(blocks), kBwdBlock, 0, stream()>>>(a, total, make_fastdiv(chunks), backwards);
+    kernel<<<static_cast<unsigned>(blocks), kBlock, 0, stream()>>>(a, total, make_fastdiv(chunks), backwards);
     return launch_rc();
 }
 int logprobs_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
     if (a.K <= 64) return launch_bwd<4>(a, total, backwards);
     if (a.K <= 256) return launch_bwd<16>(a, total, backwards);
     if (a.K <= 1024) return launch_bwd<64>(a, total, backwards);
-    return launch_bwd<256>(a, total, backwards);
+    return launch_bwd<kBwdLong>(a, total, backwards);
 }
 
 // ── paired log ratios ────────────────────────────────────────────────────
@@ -232,14 +232,14 @@ __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(PairArgs a)
 // work is less than the launches (2 pairs, 90 tokens x 256: 16 -> 7 us).
 constexpr int kSmallBlock = 1024, kSmallRounds = 4;
 template <int G>
-__global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHead<false> head, PairArgs pairs, BwdArgs bwd,
+__global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHead<false, true> head, PairArgs pairs, BwdArgs bwd,
                                                                        PairTotal total) {
     constexpr int kTeams = kSmallBlock / G;
     __shared__ ColumnShared<G> shared;
     __shared__ double slots[kSmallBlock / kWave];
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
     for (int n = threadIdx.x / G; n < bwd.N; n += kTeams)
-        token_column<LogprobHead<false>, G, kGroupQuads, false, false>(head, team, shared, nullptr, n, nullptr,
+        token_column<LogprobHead<false, true>, G, kGroupQuads, false, false>(head, team, shared, nullptr, n, nullptr,
                                                                        bwd.x + n * bwd.ld, bwd.K);
     __syncthreads();
     const Team<kWave> wave{static_cast<int>(threadIdx.x % kWave)};
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHe
     fold_parts<kSmallBlock>(total.out, total.losses, total.pairs, total.scale, slots);
 }
 template <int G>
-int launch_small(const LogprobHead<false>& head, const PairArgs& pairs, const BwdArgs& bwd, const PairTotal& total) {
+int launch_small(const LogprobHead<false, true>& head, const PairArgs& pairs, const BwdArgs& bwd, const PairTotal& total) {
     preference_small_kernel<G><<<1, kSmallBlock, 0, stream()>>>(head, pairs, bwd, total);
     return launch_rc();
 }
@@ -269,7 +269,8 @@ JZ_API int jzhip_token_logprobs(float* logp, float* entropy, float* stats, float
                                 const int32_t* labels, int K, int N, int ld) {
     if (!token_args_ok(logits, nullptr, scratch, K, N, ld, ld) || !labels || !scratch || (!logp && !entropy && !stats))
         return -1;
-    return logprobs(logp, entropy, stats, nullptr, scratch, logits, labels, K, N, static_cast<size_t>(ld));
+    auto run = entropy ? logprobs<true, false> : logprobs<false, false>;
+    return run(logp, entropy, stats, nullptr, scratch, logits, labels, K, N, static_cast<size_t>(ld));
 }
 
 JZ_API int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const float* logits, const int32_t* labels,
@@ -309,13 +310,13 @@ JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, f
         const int lanes = K <= 64 ? 4 : K <= 256 ? 16 : 64;
         if (N <= kSmallRounds * kSmallBlock / lanes) {
             begins(0, pairs);
-            const LogprobHead<false> head{exp_scale(1.0), labels, logp, nullptr, stats, N, exact};
+            const LogprobHead<false, true> head{exp_scale(1.0), labels, logp, nullptr, stats, N, exact};
             if (lanes == 4) return launch_small<4>(head, args, bwd, total);
             if (lanes == 16) return launch_small<16>(head, args, bwd, total);
             return launch_small<64>(head, args, bwd, total);
         }
     }
-    int rc = logprobs(logp, nullptr, stats, exact, scratch, logits, labels, K, N, ldx);
+    int rc = logprobs<false, true>(logp, nullptr, stats, exact, scratch, logits, labels, K, N, ldx);
     for (int at = 0; rc == 0 && at < pairs; at += kPairsPerLaunch) {
         const int n = pairs - at < kPairsPerLaunch ? pairs - at : kPairsPerLaunch;
         begins(at, n);

@@ -10,10 +10,11 @@
 // What bounds all of them is memory: 8 bytes per logit against about a dozen vector
 // instructions.
 //
-// Accuracy: a thread adds sixteen exponentials in fp32, those that are 1 apart, and everything
-// further in 64 bits.  Losses over many tokens cancel (the reward of an answer is a sum of
-// small differences of log-probabilities), so an error of a few 1e-8 per token shows in
-// them: sums in fp32 alone made rewards ten times less exact.  What happens once per column (log s,
+// Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.
+// Where a loss over many tokens cancels (the reward of an answer is a sum of small differences
+// of log-probabilities, and an error of a few 1e-8 per token shows in it), those that are 1
+// are counted apart: where one logit stands out, what the others add to its 1 is what log s
+// is made of, and fp32 rounds it at 2^-24 (Head::kExact; reading alone 61 -> 65 us for 400 MB).  What happens once per column (log s,
 // ratios, divergences) is done in 64 bits too.
 #pragma once
 
@@ -21,6 +22,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace jz {
 
@@ -242,7 +244,7 @@ __device__ __forceinline__ float quad_max(const Quad& v) { return fmaxf(fmaxf(v.
 // only a factor exp(m_group - m) once that is known.
 constexpr int kGroupQuads = 4;
 struct Group {
-    float m, s, ones, et, rest;   // s: of the exponentials below 1, ones: how many are 1
+    float m, s, ones, et, rest;   // exact heads: s of the exponentials below 1, ones: how many are 1
 };
 // x: the group's logits; without the entropy they become e_i relative to the group.  known(k): the
 // teacher's entries among quad k.
@@ -260,11 +262,10 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
         const float t0 = x[k].x - shift, t1 = x[k].y - shift, t2 = x[k].z - shift, t3 = x[k].w - shift;
         const float e0 = exp_shifted(t0, scale), e1 = exp_shifted(t1, scale);
         const float e2 = exp_shifted(t2, scale), e3 = exp_shifted(t3, scale);
-        // Where one logit stands out, what the others add to its 1 is what log s is made of, and fp32 would
-        // round it at 2^-24: the ones are counted apart (an exponential is its own fraction otherwise).
         all[k] = (e0 + e1) + (e2 + e3);
-        s[k] = (__builtin_amdgcn_fractf(e0) + __builtin_amdgcn_fractf(e1)) +
-               (__builtin_amdgcn_fractf(e2) + __builtin_amdgcn_fractf(e3));
+        if constexpr (Head::kExact)   // (an exponential below 1 is its own fraction)
+            s[k] = (__builtin_amdgcn_fractf(e0) + __builtin_amdgcn_fractf(e1)) +
+                   (__builtin_amdgcn_fractf(e2) + __builtin_amdgcn_fractf(e3));
         if constexpr (Head::kEntropy)
             et[k] = (e0 * fmaxf(t0, -200.f) + e1 * fmaxf(t1, -200.f)) + (e2 * fmaxf(t2, -200.f) + e3 * fmaxf(t3, -200.f));
         else
@@ -274,8 +275,12 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
             rest[k] = ((b & 1u ? 0.f : e0) + (b & 2u ? 0.f : e1)) + ((b & 4u ? 0.f : e2) + (b & 8u ? 0.f : e3));
         }
     }
-    g.s = (s[0] + s[1]) + (s[2] + s[3]);
-    g.ones = rintf(((all[0] + all[1]) + (all[2] + all[3])) - g.s);
+    g.s = (all[0] + all[1]) + (all[2] + all[3]);
+    if constexpr (Head::kExact) {
+        const float below = (s[0] + s[1]) + (s[2] + s[3]);
+        g.ones = rintf(g.s - below);
+        g.s = below;
+    }
     if constexpr (Head::kEntropy) g.et = (et[0] + et[1]) + (et[2] + et[3]);
     if constexpr (Head::kRest) g.rest = (rest[0] + rest[1]) + (rest[2] + rest[3]);
     return g;
@@ -294,7 +299,7 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
 }
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
-    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s) * (1.0 + kExpShort),
+    ColumnSums more{g.m, (Head::kExact ? static_cast<double>(g.ones) : 0.0) + static_cast<double>(g.s) * (1.0 + kExpShort),
                     static_cast<double>(g.et), static_cast<double>(g.rest)};
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
@@ -307,7 +312,7 @@ __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const E
 template <class Head>
 __device__ __forceinline__ Group take_one(float x, bool known) {
     const float e = x == -INFINITY ? 0.f : x - x + 1.f;   // exp of its shift from itself; a NaN or +inf shows
-    return Group{x, 0.f, e, 0.f, known ? 0.f : e};
+    return Group{x, Head::kExact ? 0.f : e, e, 0.f, known ? 0.f : e};
 }
 
 // The compiler would interleave the independent work of an unrolled loop and spill what it
@@ -324,19 +329,20 @@ __device__ __forceinline__ void correct_label(int label, float m, const Grad& f,
     out[label] = grad_value<LINEAR>(t, exp_shifted(t, scale), f.a, f.b) + f.g;
 }
 
-// Where the quads of a tile lie: up to NV per thread from quad `base` on, those of a wave one
-// stretch of memory (a wave that strides by the workgroup's width instead: 5 % slower, 193
-// against 182 us for one read and one write of 512 MB each).
-template <int G, int NV>
+// Where the quads of a tile lie: up to NV per thread from quad `base` on.  STRETCH: those of a
+// wave are one stretch of memory, which suits the writing sweep (one read and one write of
+// 512 MB each: 182 us, 193 with a wave that strides by the workgroup's width) and not reading
+// alone (512 MB less a quarter: 69 us against 66).
+template <int G, int NV, bool STRETCH>
 struct Tile {
-    int first, count;   // of this thread: quads first + k*kLanes, k < count
+    int first, count;
     static constexpr int kLanes = Team<G>::kLanes;
     __device__ __forceinline__ Tile(int rank, int base, int quads) {
         const int n = (quads - base + G - 1) / G;
         count = n < NV ? n : NV;
-        first = base + rank / kLanes * kLanes * count + rank % kLanes;
+        first = base + (STRETCH ? rank / kLanes * kLanes * count + rank % kLanes : rank);
     }
-    __device__ __forceinline__ int at(int k) const { return first + k * kLanes; }
+    __device__ __forceinline__ int at(int k) const { return first + k * (STRETCH ? kLanes : G); }
     __device__ __forceinline__ bool has(int k, int quads) const { return k < count && at(k) < quads; }
 };
 
@@ -360,7 +366,8 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     constexpr bool kKeepMax = Head::kWrites && !Head::kEntropy;   // the kept exponentials are relative to it
     const Span span = span_of<(G > 4)>(p, K);   // (by the logits: values are the same bits with and without a gradient)
     const float* const body = p + span.skew;
-    const Tile<G, NV> mine(team.rank, 0, span.quads);
+    using ColumnTile = Tile<G, NV, Head::kWrites>;
+    const ColumnTile mine(team.rank, 0, span.quads);
     bool live = head.live(col, K);
     Quad v[kGroups][kGroupQuads];
     float group_max[kGroups];
@@ -369,7 +376,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     typename Head::Early early{};
     if (live) {
         const unsigned* bits = nullptr;
-        auto take = [&](Quad (&x)[kGroupQuads], const Tile<G, NV>& tile, int first) {
+        auto take = [&](Quad (&x)[kGroupQuads], const ColumnTile& tile, int first) {
             const Group g = take_group<Head>(x, head.scale, [&](int k) {
                 const int q = tile.at(first + k);
                 return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));   // (nothing counts behind the column)
@@ -400,15 +407,18 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
             team.sync();   // the entries are marked
             bits = head.bits(own);
         }
+        auto load = [&](const ColumnTile& tile, auto cached) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                Quad& x = v[k / kGroupQuads][k % kGroupQuads];
+                x = Quad(-INFINITY);
+                if (tile.has(k, span.quads)) x = load_quad<NT && !decltype(cached)::value>(body + 4 * static_cast<size_t>(tile.at(k)));
+            }
+        };
         if constexpr (STREAM) {
             for (int base = kTile; base < span.quads; base += kTile) {
-                const Tile<G, NV> tile(team.rank, base, span.quads);
-#pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    Quad& x = v[k / kGroupQuads][k % kGroupQuads];
-                    x = Quad(-INFINITY);
-                    if (tile.has(k, span.quads)) x = load_quad<NT && !Head::kWrites>(body + 4 * static_cast<size_t>(tile.at(k)));
-                }
+                const ColumnTile tile(team.rank, base, span.quads);
+                load(tile, std::bool_constant<Head::kWrites>{});   // read again later
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
                     take(v[i], tile, i * kGroupQuads);
@@ -416,12 +426,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
                 }
             }
         }
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            Quad& x = v[k / kGroupQuads][k % kGroupQuads];
-            x = Quad(-INFINITY);
-            if (mine.has(k, span.quads)) x = load_quad<NT>(body + 4 * static_cast<size_t>(mine.at(k)));
-        }
+        load(mine, std::false_type{});
         if (team.rank < span.odd) last = p[span.single(team.rank)];
         if constexpr (Head::kTeacher && !kTeacherFirst) teach();
         if constexpr (!STREAM && Head::kRest) {
@@ -497,7 +502,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     if constexpr (STREAM) {
         constexpr int kQuads = 8, kStep = kQuads * G;
         for (int base = (span.quads - 1) / kStep * kStep; base >= kTile; base -= kStep) {
-            const Tile<G, kQuads> tile(team.rank, base, span.quads);
+            const Tile<G, kQuads, true> tile(team.rank, base, span.quads);
             Quad x[kQuads];
 #pragma unroll
             for (int k = 0; k < kQuads; ++k) {
@@ -797,10 +802,11 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
     const int rc = launch_rc();
     return rc || FOLD ? rc : launch_token_fold(sums, N);
 }
+// (what an exact head reads, the gradient's sweep reads again: it leaves the caches be)
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                          size_t ldd) {
-    if (!head.read_again() && streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
+    if (!Head::kExact && streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
         return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
     return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }

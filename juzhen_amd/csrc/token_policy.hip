@@ -14,7 +14,7 @@ namespace {
 
 template <bool ENTROPY>
 struct PolicyHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true, kExact = false;
     struct Early {
         float x, old, ref, adv, w;   // x: the label's logit
     };
@@ -26,7 +26,6 @@ struct PolicyHead {
     int N;
 
     __host__ __device__ size_t team_bytes(int) const { return 0; }
-    bool read_again() const { return false; }
     __device__ bool live(size_t col, int K) const {
         return label_scored(labels[col], K) && !(weight && weight[col] == 0.f);
     }
