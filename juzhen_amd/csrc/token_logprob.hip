@@ -175,17 +175,20 @@ struct PairArgs {
     int K, N, kind, average;
     float beta, smoothing, scale;
 };
-// One pair by one team; slots: 4*kWaves values in LDS.
-template <class T>
-__device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int pair, double* slots) {
+// One pair by one team; slots: 4*kWaves values in LDS.  token(n, v): whether token n is scored, and its
+// log-probability; put(n, g): its dl/dlogp.
+template <class T, class Token, class Put>
+__device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int pair, double* slots, double* loss_out,
+                                          Token token, Put put) {
     double reward[2], share[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int lo = a.begins.at[2 * pair + k], hi = a.begins.at[2 * pair + k + 1];
         double gain = 0.0, count = 0.0;
         for (int n = lo + team.rank; n < hi; n += T::kSize) {
-            if (!label_scored(a.labels[n], a.K) || a.stats[static_cast<size_t>(a.N) + n] == 0.f) continue;
-            gain += a.logp[n] - (a.ref ? static_cast<double>(a.ref[n]) : 0.0);
+            double v;
+            if (!token(n, v)) continue;
+            gain += v - (a.ref ? static_cast<double>(a.ref[n]) : 0.0);
             count += 1.0;
         }
         gain = team.reduce(gain, AddOp{}, slots + 2 * k * T::kWaves);
@@ -196,7 +199,7 @@ __device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int 
     const double h = reward[0] - reward[1];
     double loss, slope;   // of h; the comparisons are written so that a NaN stays one
     if (a.kind == kSigmoid) {
-        const double z = exp(-fabs(h)), tail = log1p(z);
+        const double z = exp64(-fabs(h)), tail = z < 1e-5 ? z - 0.5 * z * z : log64(1.0 + z);   // log(1 + z)
         const double down = (h >= 0.0 ? z : 1.0) / (1.0 + z), up = (h >= 0.0 ? 1.0 : z) / (1.0 + z);   // sigma(-h), sigma(h)
         const double sm = static_cast<double>(a.smoothing);
         loss = (1.0 - sm) * (tail + (h >= 0.0 ? 0.0 : -h)) + sm * (tail + (h >= 0.0 ? h : 0.0));
@@ -212,42 +215,126 @@ __device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int 
     if (team.rank == 0) {
         a.rewards[2 * pair] = static_cast<float>(reward[0]);
         a.rewards[2 * pair + 1] = static_cast<float>(reward[1]);
-        a.losses[pair] = loss;
+        *loss_out = loss;
     }
     if (!a.g) return;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const double v = (k ? -slope : slope) * share[k] * static_cast<double>(a.beta) * static_cast<double>(a.scale);
         for (int n = a.begins.at[2 * pair + k] + team.rank; n < a.begins.at[2 * pair + k + 1]; n += T::kSize)
-            a.g[n] = static_cast<float>(v);
+            put(n, static_cast<float>(v));
     }
 }
 constexpr int kPairBlock = 256;
 __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(PairArgs a) {
     __shared__ double slots[4 * kPairBlock / kWave];
-    take_pair(a, Team<kPairBlock>{static_cast<int>(threadIdx.x)}, blockIdx.x, slots);
+    take_pair(
+        a, Team<kPairBlock>{static_cast<int>(threadIdx.x)}, blockIdx.x, slots, a.losses + blockIdx.x,
+        [&](int n, double& v) {
+            v = a.logp[n];
+            return label_scored(a.labels[n], a.K) && a.stats[static_cast<size_t>(a.N) + n] != 0.f;
+        },
+        [&](int n, float g) { a.g[n] = g; });
 }
 
-// Short sequences over few classes: all three steps and the sum in one workgroup, since the
-// work is less than the launches (2 pairs, 90 tokens x 256: 16 -> 7 us).
-constexpr int kSmallBlock = 1024, kSmallRounds = 4;
+// Short sequences over few classes: one workgroup keeps every column in registers from the
+// log-probabilities to the gradient, with the pairs between two barriers.  The work is less
+// than the launches and the round trips to memory of the general way (2 pairs, 90 tokens x 256:
+// 4 launches 16 us; one workgroup that reads again for the gradient 10 us; this 6 us).
+constexpr int kSmallBlock = 1024, kSmallRounds = 2;
 template <int G>
-__global__ __launch_bounds__(kSmallBlock) void preference_small_kernel(LogprobHead<false, true> head, PairArgs pairs, BwdArgs bwd,
-                                                                       PairTotal total) {
+__global__ __launch_bounds__(kSmallBlock, 4) void preference_small_kernel(LogprobHead<false, true> head, PairArgs pairs,
+                                                                          BwdArgs a, PairTotal total) {
+    using Head = LogprobHead<false, true>;
     constexpr int kTeams = kSmallBlock / G;
-    __shared__ ColumnShared<G> shared;
-    __shared__ double slots[kSmallBlock / kWave];
+    __shared__ double logp[kSmallRounds * kTeams], losses[kPairsPerLaunch];
+    __shared__ float up[kSmallRounds * kTeams];
+    __shared__ bool scored[kSmallRounds * kTeams];
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
-    for (int n = threadIdx.x / G; n < bwd.N; n += kTeams)
-        token_column<LogprobHead<false, true>, G, kGroupQuads, false, false>(head, team, shared, nullptr, n, nullptr,
-                                                                       bwd.x + n * bwd.ld, bwd.K);
+    const int slot = threadIdx.x / G;
+    Quad v[kSmallRounds][kGroupQuads];
+    float last[kSmallRounds], picked[kSmallRounds], group[kSmallRounds];
+    int label[kSmallRounds];
+    ColumnSums c[kSmallRounds];
+    bool live[kSmallRounds];
+    Span span[kSmallRounds];
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+        const int n = slot + r * kTeams;
+        label[r] = n < a.N ? a.labels[n] : -1;
+    }
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+        const float* p = a.x + (slot + r * kTeams) * a.ld;
+        live[r] = label_scored(label[r], a.K);
+        span[r] = span_of<(G > 4)>(p, a.K);
+        last[r] = -INFINITY;
+        picked[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kGroupQuads; ++k) {
+            const int q = team.rank + k * G;
+            v[r][k] = Quad(-INFINITY);
+            if (live[r] && q < span[r].quads) v[r][k] = load_quad<false>(p + span[r].skew + 4 * q);
+        }
+        if (live[r]) picked[r] = p[label[r]];
+        if (live[r] && team.rank < span[r].odd) last[r] = p[span[r].single(team.rank)];
+    }
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+        const int n = slot + r * kTeams;
+        if (n >= a.N) continue;
+        c[r] = ColumnSums{-INFINITY, 0.0, 0.0, 0.0};
+        const Group g = take_group<Head>(v[r], head.scale, [](int) { return 0u; });
+        group[r] = g.m;
+        add_group<Head>(c[r], g, head.scale);
+        if (team.rank < span[r].odd) add_group<Head>(c[r], take_one<Head>(last[r], false), head.scale);
+        scale_sums<Head>(c[r], team.reduce(c[r].m, LargerOp{}, static_cast<float*>(nullptr)), head.scale);
+        c[r].s = team.reduce(c[r].s, AddOp{}, static_cast<double*>(nullptr));
+        live[r] = live[r] && !(c[r].m == -INFINITY && c[r].s == c[r].s);
+        const double lp = live[r] ? log_prob(picked[r], c[r]) : 0.0;
+        if (team.rank == 0) {
+            head.write(n, lp, 0.f, live[r] ? c[r].m : 0.f, live[r] ? static_cast<float>(c[r].s) : 0.f);
+            logp[n] = lp;
+            scored[n] = live[r];
+        }
+        __builtin_amdgcn_sched_barrier(0);   // one round's registers at a time
+    }
     __syncthreads();
     const Team<kWave> wave{static_cast<int>(threadIdx.x % kWave)};
-    for (int p = threadIdx.x / kWave; p < total.pairs; p += kSmallBlock / kWave) take_pair(pairs, wave, p, nullptr);
+    for (int p = threadIdx.x / kWave; p < total.pairs; p += kSmallBlock / kWave)
+        take_pair(
+            pairs, wave, p, nullptr, losses + p,
+            [&](int n, double& x) {
+                x = logp[n];
+                return scored[n];
+            },
+            [&](int n, float g) { up[n] = g; });
     __syncthreads();
-    if (bwd.d)
-        for (int n = threadIdx.x / G; n < bwd.N; n += kTeams) bwd_span<G, kGroupQuads, false>(bwd, team, n, 0);
-    fold_parts<kSmallBlock>(total.out, total.losses, total.pairs, total.scale, slots);
+    if (threadIdx.x < kWave) fold_parts<kWave>(total.out, losses, total.pairs, total.scale, nullptr);
+    if (!a.d) return;
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r) {
+        const int n = slot + r * kTeams;
+        if (n >= a.N) continue;
+        float* out = a.d + n * a.ldd;
+        const float g = live[r] ? up[n] : 0.f;
+        const bool write = live[r] && g != 0.f;
+        // (a maximum of -inf that is scored holds a NaN)
+        const float f = write ? static_cast<float>(-static_cast<double>(g) / c[r].s) : 0.f;
+        const float fg = write ? (c[r].m == -INFINITY ? 1.f : exp_shifted(group[r] - c[r].m, head.scale)) * f : 0.f;
+#pragma unroll
+        for (int k = 0; k < kGroupQuads; ++k) {
+            const int q = team.rank + k * G;
+            const Quad e = v[r][k];
+            if (q < span[r].quads)
+                store_quad<false>(out + span[r].skew + 4 * q,
+                                  write ? Quad{e.x * fg, e.y * fg, e.z * fg, e.w * fg} : Quad(0.f));
+        }
+        if (team.rank < span[r].odd)
+            out[span[r].single(team.rank)] = write ? exp_shifted(last[r] - c[r].m, head.scale) * f : 0.f;
+        team.sync();
+        if (write && team.rank == 0) correct_label<false>(label[r], c[r].m, Grad{f, 0.f, g, picked[r]}, head.scale, out);
+    }
 }
 template <int G>
 int launch_small(const LogprobHead<false, true>& head, const PairArgs& pairs, const BwdArgs& bwd, const PairTotal& total) {

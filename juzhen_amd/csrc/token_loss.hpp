@@ -520,10 +520,10 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     if (team.leads()) head.correct(team.lead(), own, col, c.m, f, out);
 }
 
-// out[k] = scale * sum_i part[k*stride + i] by a workgroup of BLOCK threads, in 64 bits in a fixed order.
+// *out = scale * sum of p[0 ... n) by a wave or a workgroup of BLOCK threads, in 64 bits in a fixed order.
 template <int BLOCK, class T>
 __device__ __forceinline__ void fold_parts(float* out, const T* p, int n, double scale, double* slots) {
-    const Team<BLOCK> team{static_cast<int>(threadIdx.x)};
+    const Team<BLOCK> team{static_cast<int>(threadIdx.x % BLOCK)};
     double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
     int i = team.rank;
     for (; i + 3 * BLOCK < n; i += 4 * BLOCK) {
@@ -565,12 +565,11 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
         token_column<Head, G, NV, NT, STREAM>(head, team, shared, dynamic + static_cast<size_t>(slot) * head.team_bytes(K),
                                               col, d ? d + col * ldd : nullptr, x + col * ld, K);
     }
-    if constexpr (FOLD) {
-        __shared__ double slots[BLOCK / kWave];
-        for (int k = 0; k < sums.count; ++k) {
-            __syncthreads();   // the parts are written; the slots read
-            fold_parts<BLOCK>(sums.out + k, sums.part + static_cast<size_t>(k) * N, N, 1.0, slots);
-        }
+    if constexpr (FOLD) {   // a wave per sum
+        __syncthreads();
+        const int k = threadIdx.x / kWave;
+        if (k < sums.count)
+            fold_parts<kWave>(sums.out + k, sums.part + static_cast<size_t>(k) * N, N, 1.0, nullptr);
     }
 }
 
