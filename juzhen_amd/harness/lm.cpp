@@ -112,6 +112,15 @@ struct Model {
     int32_t* stage[2] = {};
     void* staged[2] = {};
     unsigned batches = 0;
+    // Training objectives other than cross-entropy (jzlm_policy, jzlm_preference, jzlm_distill): per-token
+    // inputs and results on the device, made by the first call that needs them.
+    struct {
+        int32_t* labels = nullptr;
+        float *in[4] = {}, *logp = nullptr, *stats = nullptr, *rewards = nullptr, *sums = nullptr;
+        float *teacher = nullptr, *scratch = nullptr;
+        int32_t* ids = nullptr;
+        int top = 0;   // entries per token the last three have room for
+    } obj;
     float* io = nullptr;  // dense staging for get/set of strided views
     size_t io_floats = 0;
     int iteration = 1;
@@ -266,12 +275,12 @@ struct Lanes {
     }
 };
 
-void backward(Model& M, bool update) {
+// From dlogits (the head's loss has been formed) to every parameter's gradient.
+void backward_from_logits(Model& M, bool update) {
     const Config& c = M.c;
     const int d = c.d_model, N = M.N, ff = c.d_ff, V = c.vocab;
     const float* xL = M.blocks.empty() ? M.x0 : M.blocks.back().out;
     Lanes lanes(M);
-    M.ck(jzhip_softmax_xent(M.loss, M.dlogits, M.logits, M.targets, V, N, V));
     float* dy = M.dx[0];  // gradient w.r.t. the current block's output
     if (c.tied) {
         gemm(M, M.t[M.E].w, false, M.dlogits, false, dy, d, N, V);       // E * dlogits
@@ -356,6 +365,48 @@ void backward(Model& M, bool update) {
         step_group(M, kPlain);
         M.iteration++;
     }
+}
+
+void backward(Model& M, bool update) {
+    M.ck(jzhip_softmax_xent(M.loss, M.dlogits, M.logits, M.targets, M.c.vocab, M.N, M.c.vocab));
+    backward_from_logits(M, update);
+}
+
+// Room for the objectives' arrays; `top` entries per token for distillation.
+bool objective(Model& M, int top) {
+    auto& o = M.obj;
+    const size_t N = static_cast<size_t>(M.N);
+    if (!o.logp) {
+        o.labels = reinterpret_cast<int32_t*>(M.alloc(N));
+        for (float*& p : o.in) p = M.alloc(N);
+        o.logp = M.alloc(N);
+        o.stats = M.alloc(2 * N);
+        o.rewards = M.alloc(N + 1);   // at most a sequence per token
+        o.sums = M.alloc(4);
+    }
+    if (!o.scratch || top > o.top) {
+        // outgrown buffers stay with the model until it is destroyed
+        o.scratch = M.alloc(jzhip_token_scratch_floats(M.N, top));
+        if (top > 0) {
+            o.teacher = M.alloc(N * top);
+            o.ids = reinterpret_cast<int32_t*>(M.alloc(N * top));
+        }
+        o.top = top;
+    }
+    return M.rc == 0;
+}
+// The labels to score: the targets of the batch, or the caller's.
+const int32_t* objective_labels(Model& M, const int32_t* host) {
+    if (!host) return M.targets;
+    M.ck(jzhip_memcpy_h2d(reinterpret_cast<float*>(M.obj.labels), reinterpret_cast<const float*>(host),
+                          static_cast<size_t>(M.N)));
+    return M.obj.labels;
+}
+// Device copy of a per-token host array, or NULL.
+const float* objective_input(Model& M, int slot, const float* host) {
+    if (!host) return nullptr;
+    M.ck(jzhip_memcpy_h2d(M.obj.in[slot], host, static_cast<size_t>(M.N)));
+    return M.obj.in[slot];
 }
 
 }  // namespace
@@ -541,6 +592,78 @@ JZLM_API int jzlm_forward(void* h) {
 JZLM_API int jzlm_backward(void* h, int update) {
     Model* M = static_cast<Model*>(h);
     backward(*M, update != 0);
+    return M->rc;
+}
+// Training objectives in the place of cross-entropy.  forward must have run; per-token host arrays
+// hold N = batch * seq values (token n = b * seq + s), optional ones may be NULL; labels: the ids
+// to score, NULL for the batch's targets, -1 for a token that is not.  Each call forms the loss
+// (jzlm_loss), the gradients of all parameters, and applies the optimiser when update != 0; a call
+// that is refused (-1) changes nothing.
+
+// log-probabilities of the labels under the model as it is: the reference and the sampling policy
+JZLM_API int jzlm_logprobs(void* h, const int32_t* labels, float* host_logp) {
+    Model* M = static_cast<Model*>(h);
+    if (!host_logp) return -1;
+    if (!objective(*M, 0)) return M->rc;
+    const int32_t* l = objective_labels(*M, labels);
+    M->ck(jzhip_token_logprobs(M->obj.logp, nullptr, nullptr, M->obj.scratch, M->logits, l, M->c.vocab, M->N, M->c.vocab));
+    M->ck(jzhip_memcpy_d2h(host_logp, M->obj.logp, static_cast<size_t>(M->N)));
+    return M->rc;
+}
+// jzhip_policy_loss; host_sums (4 floats, may be NULL) as there
+JZLM_API int jzlm_policy(void* h, const int32_t* labels, const float* old_logp, const float* ref_logp,
+                         const float* advantage, const float* weight, float clip_low, float clip_high, float kl_coef,
+                         float entropy_coef, int update, float* host_sums) {
+    Model* M = static_cast<Model*>(h);
+    if (!old_logp || !advantage) return -1;
+    if (!objective(*M, 0)) return M->rc;
+    const int V = M->c.vocab;
+    const int32_t* l = objective_labels(*M, labels);
+    const float *o = objective_input(*M, 0, old_logp), *r = objective_input(*M, 1, ref_logp),
+                *a = objective_input(*M, 2, advantage), *w = objective_input(*M, 3, weight);
+    const int rc = jzhip_policy_loss(M->obj.sums, M->obj.logp, M->dlogits, M->obj.scratch, M->logits, l, o, r, a, w, V,
+                                     M->N, V, V, clip_low, clip_high, kl_coef, entropy_coef);
+    if (rc) return rc;
+    M->ck(jzhip_copy(M->loss, M->obj.sums, 1));
+    backward_from_logits(*M, update != 0);
+    if (host_sums) M->ck(jzhip_memcpy_d2h(host_sums, M->obj.sums, 4));
+    return M->rc;
+}
+// jzhip_preference_loss over pairs of consecutive sequences of the batch (chosen, rejected), the mean
+// over the pairs; host_rewards (batch floats, may be NULL)
+JZLM_API int jzlm_preference(void* h, const int32_t* labels, const float* ref_logp, int kind, float beta,
+                             float smoothing, int average, int update, float* host_rewards) {
+    Model* M = static_cast<Model*>(h);
+    const int V = M->c.vocab, pairs = M->c.batch / 2;
+    if (M->c.batch % 2 != 0) return -1;
+    if (!objective(*M, 0)) return M->rc;
+    const int32_t* l = objective_labels(*M, labels);
+    const float* r = objective_input(*M, 1, ref_logp);
+    std::vector<int> begin(M->c.batch + 1);
+    for (int b = 0; b <= M->c.batch; ++b) begin[b] = b * M->c.seq;
+    const int rc = jzhip_preference_loss(M->loss, M->obj.rewards, M->obj.logp, M->obj.stats, M->dlogits, M->obj.scratch,
+                                         M->logits, l, r, begin.data(), pairs, V, V, V, kind, beta, smoothing, average,
+                                         1.0f / static_cast<float>(pairs));
+    if (rc) return rc;
+    backward_from_logits(*M, update != 0);
+    if (host_rewards) M->ck(jzhip_memcpy_d2h(host_rewards, M->obj.rewards, static_cast<size_t>(M->c.batch)));
+    return M->rc;
+}
+// jzhip_distill_topk; teacher and ids: top values per token, teacher_lse and weight per token or NULL
+JZLM_API int jzlm_distill(void* h, const float* teacher, const int32_t* ids, int top, const float* teacher_lse,
+                          const float* weight, float temperature, int update) {
+    Model* M = static_cast<Model*>(h);
+    const int V = M->c.vocab;
+    if (!teacher || !ids || top <= 0 || top > 512 || top > V) return -1;
+    if (!objective(*M, top)) return M->rc;
+    const size_t n = static_cast<size_t>(M->N) * top;
+    M->ck(jzhip_memcpy_h2d(M->obj.teacher, teacher, n));
+    M->ck(jzhip_memcpy_h2d(reinterpret_cast<float*>(M->obj.ids), reinterpret_cast<const float*>(ids), n));
+    const float *z = objective_input(*M, 0, teacher_lse), *w = objective_input(*M, 1, weight);
+    const int rc = jzhip_distill_topk(M->loss, nullptr, M->dlogits, M->obj.scratch, M->logits, M->obj.teacher, M->obj.ids,
+                                      z, w, V, top, M->N, V, V, top, temperature);
+    if (rc) return rc;
+    backward_from_logits(*M, update != 0);
     return M->rc;
 }
 // one training step: forward, loss, backward, optimiser

@@ -55,6 +55,12 @@ def load():
         lib.jzlm_loss.argtypes = [C.c_void_p]
         lib.jzlm_logits.restype = C.c_int
         lib.jzlm_logits.argtypes = [C.c_void_p, C.c_void_p]
+        I, F, P = C.c_int, C.c_float, C.c_void_p
+        for name, args in (("jzlm_logprobs", [P, P, P]), ("jzlm_policy", [P] * 6 + [F] * 4 + [I, P]),
+                           ("jzlm_preference", [P] * 3 + [I, F, F, I, I, P]),
+                           ("jzlm_distill", [P] * 3 + [I, P, P, F, I])):
+            getattr(lib, name).restype = I
+            getattr(lib, name).argtypes = args
         lib.jzlm_set_iteration.argtypes = [C.c_void_p, C.c_int]
         lib.jzlm_set_overlap.argtypes = [C.c_void_p, C.c_int]
         lib.jzlm_set_overlap.restype = None
@@ -153,6 +159,53 @@ class CharLM:
 
     def backward(self, update=False):
         self._check("backward", self.lib.jzlm_backward(self.h, int(update)))
+
+    # -- objectives in the place of cross-entropy; per-token arrays are (batch, seq) or flat ----------
+
+    def _tokens(self, a, dtype=np.float32, per=1):
+        if a is None:
+            return None
+        return np.ascontiguousarray(np.asarray(a, dtype=dtype).reshape(self.tokens_per_step * per))
+
+    @staticmethod
+    def _ptr(a):
+        return None if a is None else a.ctypes.data
+
+    def logprobs(self, labels=None):
+        """log p of the labels (default: the batch's targets; -1: not scored, 0) after forward()."""
+        lab, out = self._tokens(labels, np.int32), np.empty(self.tokens_per_step, np.float32)
+        self._check("logprobs", self.lib.jzlm_logprobs(self.h, self._ptr(lab), out.ctypes.data))
+        return out
+
+    def backward_policy(self, old_logp, advantage, ref_logp=None, weight=None, labels=None, clip_low=0.2, clip_high=0.2,
+                        kl_coef=0.0, entropy_coef=0.0, update=False):
+        """Gradients of the clipped policy loss (see jzhip_policy_loss); returns its four sums."""
+        lab, old, adv, ref, w = (self._tokens(labels, np.int32), self._tokens(old_logp), self._tokens(advantage),
+                                 self._tokens(ref_logp), self._tokens(weight))
+        sums = np.empty(4, np.float32)
+        self._check("policy", self.lib.jzlm_policy(self.h, self._ptr(lab), self._ptr(old), self._ptr(ref), self._ptr(adv),
+                                                   self._ptr(w), clip_low, clip_high, kl_coef, entropy_coef, int(update),
+                                                   sums.ctypes.data))
+        return sums
+
+    def backward_preference(self, ref_logp=None, labels=None, kind="sigmoid", beta=0.1, smoothing=0.0, average=False,
+                            update=False):
+        """Gradients of the paired log-ratio loss, sequences 2p (chosen) and 2p + 1 (rejected) of the
+        batch being pair p; returns the rewards of the sequences."""
+        lab, ref = self._tokens(labels, np.int32), self._tokens(ref_logp)
+        rewards = np.empty(self.cfg.batch, np.float32)
+        self._check("preference", self.lib.jzlm_preference(
+            self.h, self._ptr(lab), self._ptr(ref), ("sigmoid", "hinge", "squared").index(kind), beta, smoothing,
+            int(average), int(update), rewards.ctypes.data))
+        return rewards
+
+    def backward_distill(self, teacher, ids, teacher_lse=None, weight=None, temperature=1.0, update=False):
+        """Gradients of the divergence from a teacher's largest logits: teacher and ids are (..., top)."""
+        top = np.asarray(ids).shape[-1]
+        t, i = self._tokens(teacher, np.float32, top), self._tokens(ids, np.int32, top)
+        z, w = self._tokens(teacher_lse), self._tokens(weight)
+        self._check("distill", self.lib.jzlm_distill(self.h, self._ptr(t), self._ptr(i), top, self._ptr(z), self._ptr(w),
+                                                     temperature, int(update)))
 
     def step(self):
         self._check("step", self.lib.jzlm_step(self.h))
