@@ -445,9 +445,11 @@ int jzhip_softmax_xent_dense(float* loss_out, float* dlogits, const float* logit
  *   - dlogits (K x N, leading dimension ldd) may be NULL where only values are wanted, and
  *     may be logits itself with ldd == ld; otherwise outputs overlap no input.  ldd - K
  *     entries behind each column are left as they are.
- *   - sums over a column are kept in fp32 and every per-token quantity derived from them
- *     (log-probability, ratio, divergence) and every sum over tokens in 64 bits, all in a
- *     fixed order: equal inputs give equal bits.
+ *   - sixteen exponentials are added in fp32, everything further in 64 bits, as are a token's
+ *     quantities (log-probability, ratio, divergence) and the sums over tokens, all in a fixed
+ *     order: the same call on the same buffers gives the same bits, and values are the same
+ *     with dlogits as without.  (Another address modulo 16 bytes groups a column differently.)
+ *   - K up to 2^28, N and ld as int allows; offsets are 64 bits wide.
  *   - scratch: caller-provided, 16-byte aligned, jzhip_token_scratch_floats(N, top) =
  *     (8 + top) * N + 2^20 floats (top: 0 but for jzhip_distill_topk; for
  *     jzhip_preference_loss N is the number of tokens).  Nothing in it outlives a call, and no
@@ -483,7 +485,7 @@ int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* scratch,
  * sequence s is columns [seq_begin[s], seq_begin[s+1]), 2p the chosen and 2p + 1 the rejected
  * answer of pair p; a sequence may be empty.  The columns behind the last sequence are not
  * touched.  ref_logp: log-probabilities of the same tokens under the reference model
- * (jzhip_token_logprobs), NULL for none.
+ * (jzhip_token_logprobs), NULL for none; read for scored tokens only.
  *   R_s = beta * sum (log p(label) - ref_logp) over its scored tokens, divided by their number
  *   when average != 0 (0 if there is none);  h_p = R_2p - R_2p+1
  *   kind 0: l = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)   (smoothing < 0.5)
@@ -496,7 +498,7 @@ int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* s
                           const int32_t* labels, const float* ref_logp, const int* seq_begin,
                           int pairs, int K, int ld, int ldd, int kind, float beta,
                           float smoothing, int average, float scale);
-/* Distillation from the `top` largest logits of a teacher (at most 512): teacher and ids are
+/* Distillation from the `top` largest logits of a teacher (at most 512 and K): teacher and ids are
  * top x N with leading dimension ldt.  An id outside [0, K) is no entry (fewer than `top`
  * known), and of equal ids in a column only the first counts.  With T = temperature,
  * q_j = exp(teacher_j / T - lse), the student's p = softmax(x / T):

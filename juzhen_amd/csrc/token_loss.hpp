@@ -93,8 +93,12 @@ __device__ __forceinline__ double exp64(double v) {
     p = __builtin_amdgcn_ldexp(p, static_cast<int>(n));
     return v < -700.0 ? 0.0 : v > 709.0 ? INFINITY : p;
 }
-// exp(v) - 1 - v, which is v^2/2 + ... where the difference would cancel
-__device__ __forceinline__ double exp_tail64(double v) {
+// exp(v) - 1 and exp(v) - 1 - v; near 0, where the differences would cancel, from the series
+// (|v| < 0.06, cut after v^8/8!: 0.06^7 / 9! * 2 = 1e-14).
+struct ExpTail {
+    double minus1, tail;
+};
+__device__ __forceinline__ ExpTail exp_tail64(double v) {
     double p = 1.0 / 40320.0;
     p = fma(p, v, 1.0 / 5040.0);
     p = fma(p, v, 1.0 / 720.0);
@@ -102,7 +106,9 @@ __device__ __forceinline__ double exp_tail64(double v) {
     p = fma(p, v, 1.0 / 24.0);
     p = fma(p, v, 1.0 / 6.0);
     p = fma(p, v, 0.5) * v * v;
-    return fabs(v) < 0.06 ? p : (exp64(v) - 1.0) - v;   // 0.06^7 / 9! * 2: 1e-14
+    const double e = exp64(v) - 1.0;
+    if (fabs(v) < 0.06) return ExpTail{p + v, p};
+    return ExpTail{e, v > 709.0 ? INFINITY : e - v};
 }
 
 struct AddOp {
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
         token_column<Head, G, NV, NT, STREAM>(head, team, shared, dynamic + static_cast<size_t>(slot) * head.team_bytes(K),
                                               col, d ? d + col * ldd : nullptr, x + col * ld, K);
     }
-    if constexpr (FOLD) {   // a wave per sum
+    if constexpr (FOLD) {   // a wave per sum, of what this workgroup has written
         __syncthreads();
         const int k = threadIdx.x / kWave;
         if (k < sums.count)
@@ -743,8 +749,8 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, Tok
     }
 }
 
-// Logits of a group of columns that are read twice: the second read comes out of the
-// 256 MB memory-side cache when they and their gradient fit it.
+// Logits of a group of columns that several launches read twice: they and their gradient fit the
+// 256 MB memory-side cache.
 constexpr size_t kReadTwiceBytes = size_t(96) << 20;
 
 inline int launch_token_fold(const TokenSums& sums, int N) {
@@ -805,16 +811,21 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                          size_t ldd) {
-    if (!Head::kExact && streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
-        return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
+    if constexpr (!Head::kExact) {
+        if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
+            return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
+    }
     return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }
 // teams of one wave or less: where one workgroup holds all columns, it adds up their parts as well
+// (policy loss of 64 x 256: 9.0 us in two launches, 5.6 in one)
 template <class Head, int G, int NV>
 int launch_token_teams(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                        size_t ldd) {
-    if (NV == kGroupQuads && sums.count > 0 && N <= 1024 / G && (1024 / G) * head.team_bytes(K) <= (size_t(64) << 10))
-        return launch_token_columns_as<Head, G, kGroupQuads, 1024, false, false, true>(head, sums, d, x, K, N, ld, ldd);
+    if constexpr (Head::kWrites && NV == kGroupQuads) {
+        if (N <= 1024 / G && (1024 / G) * head.team_bytes(K) <= (size_t(64) << 10))
+            return launch_token_columns_as<Head, G, NV, 1024, false, false, true>(head, sums, d, x, K, N, ld, ldd);
+    }
     return launch_token_columns<Head, G, NV, 256, false>(head, sums, d, x, K, N, ld, ldd);
 }
 
@@ -838,7 +849,8 @@ int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch,
     if (K <= 1024) return launch_token_teams<Head, 64, 4>(head, sums, d, x, K, N, ld, ldd);
     if (K <= 2048) return launch_token_teams<Head, 64, 8>(head, sums, d, x, K, N, ld, ldd);
     if (K <= kMaxTeam) return launch_token_teams<Head, 64, 16>(head, sums, d, x, K, N, ld, ldd);
-    if (token_in_chunks(K, N, Head::kWrites) || head.team_bytes(K) > kMaxLds) return launch_token_chunks(head, sums, scratch, d, x, K, N, ld, ldd);
+    if (token_in_chunks(K, N, Head::kWrites) || head.team_bytes(K) > kMaxLds)
+        return launch_token_chunks(head, sums, scratch, d, x, K, N, ld, ldd);
     if (K <= 8192) return launch_token_columns<Head, 256, 8, 256, false>(head, sums, d, x, K, N, ld, ldd);
     if constexpr (!Head::kWrites) {
         // Values alone need no column kept; small tiles waste least of their last round: K = 24000 61 (512 x 16
@@ -849,13 +861,13 @@ int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch,
         if (K <= 16384) return launch_token_columns<Head, 256, 16, 256, false>(head, sums, d, x, K, N, ld, ldd);
         if (K <= kMaxResident) return launch_token_columns<Head, 512, 16, 512, false>(head, sums, d, x, K, N, ld, ldd);
         if (K <= 2 * kMaxResident) {
-            // Half of the column kept and two workgroups on a CU, whose loads and stores overlap: K = 48000 158
-            // (one workgroup that keeps all of it: 177), 64000 168 (169), with the teacher's rest 187 (237).  Where
-            // there is no second workgroup, the one: 256 x 64000 22 (25).
+            // Half of the column kept and two workgroups on a CU, whose loads and stores overlap: K = 48000 157
+            // (one workgroup that keeps all of it: 177), 64000 170 (169), with the teacher's rest 187 (237).  Where
+            // there is no second workgroup, the one: 256 x 64000 23 (25).
             if (N > 2 * num_cus()) return launch_token_columns<Head, 512, 16, 512, true>(head, sums, d, x, K, N, ld, ldd);
             return launch_token_columns<Head, 1024, 16, 1024, false>(head, sums, d, x, K, N, ld, ldd);
         }
-        // K = 98000 171 (512 threads: 197; 24 quads: 183), 262144 193 (215; 191), rest 230 (239; 248); chunks read
+        // K = 98000 174 (512 threads: 197; 24 quads: 183), 262144 195 (215; 191), rest 230 (239; 248); chunks read
         // twice over several launches 280.
         return launch_token_columns<Head, 1024, 16, 1024, true>(head, sums, d, x, K, N, ld, ldd);
     }

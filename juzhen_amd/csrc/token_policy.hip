@@ -57,9 +57,10 @@ struct PolicyHead {
         double loss = -(cut ? held : open), h = 0.0;
         if (ref_logp) {
             const double u = static_cast<double>(e.ref) - lp;
-            kl = exp_tail64(u);
+            const ExpTail em = exp_tail64(u);
+            kl = em.tail;
             if (kl_coef != 0.f) {
-                g -= static_cast<double>(kl_coef) * (kl + u);
+                g -= static_cast<double>(kl_coef) * em.minus1;
                 loss += static_cast<double>(kl_coef) * kl;
             }
         }

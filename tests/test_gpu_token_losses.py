@@ -232,6 +232,28 @@ def test_policy_nan_and_zero_probability(gpu, K):
 PAIRS = [(1, [3, 2]), (2, [1, 0, 0, 5]), (3, [4, 4, 9, 1, 0, 0]), (70, [1 + (7 * i) % 3 for i in range(140)])]
 
 
+@pytest.mark.parametrize("K", [3, 700, 140000])
+def test_policy_infinite_kl(gpu, K):
+    """A sampled token that the policy or the reference excludes: ratio 0 or not, KL infinite, gradient of the
+    KL term -inf times (1 - p) or its limit kl_coef, and the other tokens as ever."""
+    print(f"policy infinite kl K {K}", flush=True)
+    x = np.random.default_rng(K).normal(0, 1, (3, K)).astype(F)
+    labels = np.array([0, 1, 2], np.int32)
+    x[0, 0] = -np.inf
+    lp = ref.logprobs(x, labels)[0]
+    old, rlp, adv = np.full(3, -2.0, F), np.array([-2.0, -np.inf, lp[2] - 0.3], F), np.array([1.0, 1.0, -1.0], F)
+    lo, b = float(F(0.2)), float(F(0.1))
+    sums, lps, want, up = ref.policy(x, labels, old, rlp, adv, None, lo, lo, b, 0.0)
+    out, one, d, sc = dev_empty(4), dev_empty(3), grad_buffer(3, K), scratch(3)
+    gpu.policy_loss(dptr(out), dptr(one), dptr(d), dptr(sc), kept(columns(x, K)), kept(to_dev(labels)), kept(to_dev(old)),
+                    kept(to_dev(rlp)), kept(to_dev(adv)), None, K, 3, K, K, 0.2, 0.2, 0.1, 0.0)
+    got = take(d, 3, K, K)
+    assert to_host(out)[0] == np.inf and to_host(out)[1] == np.inf
+    same(to_host(one), lps, D(K) * U + 2 * U * np.abs(fin(lps)), "logp")
+    same(got[1:], want[1:], (np.abs(up[1:]) * (2 * D(K) + 16) + b * 4 * D(K))[:, None] * U, "gradient")
+    assert up[0] == -np.inf
+
+
 @pytest.mark.parametrize("K", [1, 13, 256, 1000, 5003, 33001, 140001])
 @pytest.mark.parametrize("pairs,lengths", PAIRS)
 @pytest.mark.parametrize("kind,sm,average", [(0, 0.0, 0), (0, 0.1, 1), (1, 0.0, 0), (2, 0.0, 1)])

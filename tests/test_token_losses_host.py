@@ -29,9 +29,12 @@ def test_scratch_size(lib):
 
 def test_logprobs_refuses(lib):
     good = [P, None, None, P, P, P, 8, 4, 8]
-    for at, bad in ((3, None), (4, None), (5, None), (6, 0), (6, -1), (7, 0), (8, 7), (0, None), (3, C.c_void_p((1 << 20) + 4))):
+    for at, bad in ((3, None), (4, None), (5, None), (6, 0), (6, -1), (6, (1 << 28) + 1), (7, 0), (8, 7), (0, None),
+                    (3, C.c_void_p((1 << 20) + 4))):
         a = list(good)
         a[at] = bad
+        if at == 6 and bad > 0:
+            a[8] = bad
         assert lib.jzhip_token_logprobs(*a) == -1, (at, bad)
     good = [P, P, Q, P, P, 8, 4, 8, 8]
     for at, bad in ((0, None), (1, None), (2, None), (3, None), (4, None), (5, 0), (6, 0), (7, 7), (8, 7)):
@@ -71,12 +74,12 @@ def test_preference_refuses(lib):
 def test_distill_refuses(lib):
     good = [P, None, Q, P, P, P, P, None, None, 8, 4, 2, 8, 8, 4, 1.0]
     nan = float("nan")
-    for at, bad in ((0, None), (3, None), (4, None), (5, None), (6, None), (9, 0), (10, 0), (10, 513), (11, 0), (12, 7),
+    for at, bad in ((0, None), (3, None), (4, None), (5, None), (6, None), (9, 0), (10, 0), (10, 513), (10, 9), (11, 0), (12, 7),
                     (13, 7), (14, 3), (15, 0.0), (15, -1.0), (15, nan), (15, 1e-4), (15, 1e4), (3, C.c_void_p((1 << 20) + 4))):
         a = list(good)
         a[at] = bad
-        if (at, bad) == (10, 513):
-            a[14] = 513
+        if at == 10 and bad > 0:
+            a[14] = bad
         assert lib.jzhip_distill_topk(*a) == -1, (at, bad)
 
 
