@@ -115,16 +115,15 @@ struct PairTotal {
 };
 // G <= 64: a column per team; else `chunks` workgroups per column
 template <int G, bool NT>
-__global__ __launch_bounds__(G > kWave ? G : kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total, FastDiv chunks,
-                                                                                bool backwards) {
+__global__ __launch_bounds__(G > kWave ? G : kBwdBlock) void logprob_bwd_kernel(BwdArgs a, PairTotal total,
+                                                                                FastDiv chunks) {
     constexpr int kBlock = G > kWave ? G : kBwdBlock, kTeams = kBlock / G;
     __shared__ double slots[kBlock / kWave];
     if (total.out && blockIdx.x == 0) fold_parts<kBlock>(total.out, total.losses, total.pairs, total.scale, slots);
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
-    int col = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
+    const int col = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
     if (kTeams > 1 && col >= a.N) return;
     const int base = kTeams > 1 ? 0 : static_cast<int>(blockIdx.x - col * chunks.d) * G;
-    if (backwards) col = a.N - 1 - col;
     bwd_span<G, (kTeams > 1 ? kGroupQuads : 1), NT>(a, team, col, base);
 }
 
@@ -136,21 +135,21 @@ int logprobs(float* logp, float* entropy, float* stats, double* exact, float* sc
 }
 
 template <int G>
-int launch_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
+int launch_bwd(const BwdArgs& a, const PairTotal& total) {
     constexpr int kBlock = G > kWave ? G : kBwdBlock, kTeams = kBlock / G;
     const int chunks = kTeams > 1 ? 1 : (a.K / 4 + G - 1) / G;
     const size_t blocks = (static_cast<size_t>(a.N) * chunks + kTeams - 1) / kTeams;
     if (blocks > 0x7fffffffull) return -1;
     const bool nt = streams_past_cache(static_cast<size_t>(a.K) * a.N * 2 * sizeof(float));
     auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
-    kernel<<<static_cast<unsigned>(blocks), kBlock, 0, stream()>>>(a, total, make_fastdiv(chunks), backwards);
+    kernel<<<static_cast<unsigned>(blocks), kBlock, 0, stream()>>>(a, total, make_fastdiv(chunks));
     return launch_rc();
 }
-int logprobs_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
-    if (a.K <= 64) return launch_bwd<4>(a, total, backwards);
-    if (a.K <= 256) return launch_bwd<16>(a, total, backwards);
-    if (a.K <= 1024) return launch_bwd<64>(a, total, backwards);
-    return launch_bwd<kBwdLong>(a, total, backwards);
+int logprobs_bwd(const BwdArgs& a, const PairTotal& total) {
+    if (a.K <= 64) return launch_bwd<4>(a, total);
+    if (a.K <= 256) return launch_bwd<16>(a, total);
+    if (a.K <= 1024) return launch_bwd<64>(a, total);
+    return launch_bwd<kBwdLong>(a, total);
 }
 
 // ── paired log ratios ────────────────────────────────────────────────────
@@ -158,6 +157,10 @@ int logprobs_bwd(const BwdArgs& a, const PairTotal& total, bool backwards) {
 // h = R_chosen - R_rejected.  The slope dl/dh scales both sequences' gradients, so every
 // log-probability of a pair is needed before the first gradient of it can be written:
 // logprobs over the columns, this kernel over the pairs, logprobs_bwd over the columns.
+// The second read is what this costs, 12 bytes per logit instead of 8, at 5.9 TB/s (4939 x
+// 32000: 70 + 6 + 185 us).  It cannot come cheaper out of the memory-side cache, which is no
+// faster than the memory (a copy of 128 MB 7.2 TB/s, of 1 GB 6.5): pairs taken in groups that
+// fit it 366 us in all, the gradient's sweep from the last column back no change.
 enum PreferenceKind { kSigmoid = 0, kHinge = 1, kSquared = 2 };
 
 constexpr int kPairsPerLaunch = 64;
@@ -225,7 +228,7 @@ __device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int 
             put(n, static_cast<float>(v));
     }
 }
-constexpr int kPairBlock = 256;
+constexpr int kPairBlock = 1024;
 __global__ __launch_bounds__(kPairBlock) void preference_pair_kernel(PairArgs a) {
     __shared__ double slots[4 * kPairBlock / kWave];
     take_pair(
@@ -365,7 +368,7 @@ JZ_API int jzhip_token_logprobs_bwd(float* dlogits, const float* dlogp, const fl
     if (!token_args_ok(logits, dlogits, nullptr, K, N, ld, ldd) || !dlogits || !dlogp || !labels || !stats) return -1;
     return logprobs_bwd(BwdArgs{dlogits, dlogp, logits, labels, stats, K, N, static_cast<size_t>(ld),
                                 static_cast<size_t>(ldd), exp_scale(1.0)},
-                        PairTotal{}, false);
+                        PairTotal{});
 }
 
 JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* stats, float* dlogits,
@@ -411,8 +414,7 @@ JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, f
         rc = launch_rc();
     }
     if (rc) return rc;
-    // the last columns read are the first ones read again: they are in the cache
-    if (dlogits) return logprobs_bwd(bwd, total, true);
+    if (dlogits) return logprobs_bwd(bwd, total);
     token_fold_kernel<double><<<1, kFoldBlock, 0, stream()>>>(loss_out, losses, pairs, 0, static_cast<double>(scale));
     return launch_rc();
 }

@@ -807,14 +807,11 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
     const int rc = launch_rc();
     return rc || FOLD ? rc : launch_token_fold(sums, N);
 }
-// (what an exact head reads, the gradient's sweep reads again: it leaves the caches be)
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                          size_t ldd) {
-    if constexpr (!Head::kExact) {
-        if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
-            return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
-    }
+    if (streams_past_cache(static_cast<size_t>(K) * N * sizeof(float) * (d ? 2 : 1)))
+        return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
     return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }
 // teams of one wave or less: where one workgroup holds all columns, it adds up their parts as well

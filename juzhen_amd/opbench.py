@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Per-kernel roofline report for the MI355X backend.
 
-    python -m juzhen_amd.opbench [--groups gemm,ew,reduce,fused,conv,broadcast,conv_implicit] [--out FILE]
+    python -m juzhen_amd.opbench [--groups gemm,ew,reduce,fused,conv,broadcast,conv_implicit,losses] [--out FILE]
 
 Every line is one C-ABI entry point at one shape: median and p95 launch time
 over 20 samples after 3 warm-ups (the reference's convention,
@@ -445,8 +445,45 @@ def bench_conv_implicit(r):
         torch.cuda.empty_cache()
 
 
+def bench_losses(r):
+    """Losses on logits; bytes: every logit of a scored token read once, every gradient written once."""
+    jz, lib = r.jz, r.lib
+
+    def ints(t):
+        return t.to(torch.int32)
+
+    # (vocabulary, tokens): the character model's batch, word pieces, odd and large vocabularies, one token
+    for K, N in ((256, 16384), (1000, 16384), (32000, 4096), (50001, 2048), (131072, 1024), (262144, 512), (262144, 1)):
+        top = 32
+        x, d = dev(N * K), dev(N * K, 0)
+        lab = ints(torch.randint(0, K, (N,), device="cuda"))
+        logp, stats, sums, up = dev(N, -3), dev(2 * N), dev(4), dev(N)
+        teacher, lse = dev(N * top), dev(N, 5.0)
+        ids = ints((torch.randint(0, K, (N, 1), device="cuda") + torch.arange(top, device="cuda") * (K // top)) % K)
+        scratch = torch.empty(lib.jzhip_token_scratch_floats(N, top), device="cuda")
+        s, one, two = f"{K}x{N}", 4 * K * N, 8 * K * N
+        r.run("losses", "jzhip_token_logprobs", s,
+              lambda: jz.token_logprobs(P(up), None, P(stats), P(scratch), P(x), P(lab), K, N, K), bytes_=one)
+        r.run("losses", "jzhip_token_logprobs_bwd", s,
+              lambda: jz.token_logprobs_bwd(P(d), P(up), P(x), P(lab), P(stats), K, N, K, K), bytes_=two)
+        for ent in (0.0, 0.01):
+            r.run("losses", "jzhip_policy_loss" + (" (entropy)" if ent else ""), s,
+                  lambda: jz.policy_loss(P(sums), None, P(d), P(scratch), P(x), P(lab), P(logp), P(logp), P(up), None, K, N,
+                                         K, K, 0.2, 0.2, 0.05, ent), bytes_=two)
+        for z in (None, lse):
+            r.run("losses", "jzhip_distill_topk top 32" + ("" if z is None else " (rest)"), s,
+                  lambda: jz.distill_topk(P(sums), None, P(d), P(scratch), P(x), P(teacher), P(ids),
+                                          None if z is None else P(z), None, K, top, N, K, K, top, 1.0), bytes_=two)
+        if N > 1:
+            begin = (C.c_int * 9)(*[N * i // 8 for i in range(9)])
+            r.run("losses", "jzhip_preference_loss 4 pairs (logits read twice)", s,
+                  lambda: jz.preference_loss(P(sums), P(up), P(logp), P(stats), P(d), P(scratch), P(x), P(lab), None, begin, 4,
+                                             K, K, K, 0, 0.1, 0.0, 0, 0.25), bytes_=two)
+        del x, d
+
+
 GROUPS = {"gemm": bench_gemm, "ew": bench_ew, "reduce": bench_reduce, "fused": bench_fused, "conv": bench_conv,
-          "broadcast": bench_broadcast, "conv_implicit": bench_conv_implicit}
+          "broadcast": bench_broadcast, "conv_implicit": bench_conv_implicit, "losses": bench_losses}
 
 
 def main():
