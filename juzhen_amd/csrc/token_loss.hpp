@@ -409,10 +409,13 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         };
         early = head.early(col, p);
         if constexpr (Head::kTeacher && kTeacherFirst) teach();
-        if constexpr (STREAM && Head::kRest) {
-            team.sync();   // the entries are marked
-            bits = head.bits(own);
-        }
+        // the entries are marked: waited for behind the first loads
+        auto marked = [&] {
+            if constexpr (Head::kRest) {
+                if (!bits) team.sync();
+                bits = head.bits(own);
+            }
+        };
         auto load = [&](const ColumnTile& tile, auto cached) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -425,6 +428,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
             for (int base = kTile; base < span.quads; base += kTile) {
                 const ColumnTile tile(team.rank, base, span.quads);
                 load(tile, std::bool_constant<Head::kWrites>{});   // read again later
+                marked();
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
                     take(v[i], tile, i * kGroupQuads);
@@ -435,10 +439,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         load(mine, std::false_type{});
         if (team.rank < span.odd) last = p[span.single(team.rank)];
         if constexpr (Head::kTeacher && !kTeacherFirst) teach();
-        if constexpr (!STREAM && Head::kRest) {
-            team.sync();
-            bits = head.bits(own);
-        }
+        marked();
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) {
             const float m = take(v[i], mine, i * kGroupQuads);
