@@ -552,3 +552,101 @@ def test_no_workspace_is_made(gpu):
     gpu.token_logprobs(kept(dev_empty(N)), None, None, kept(scratch(N)), kept(columns(x, K)), kept(to_dev(labels)), K, N, K)
     gpu.synchronize()
     assert lib.jzhip_workspace_bytes() == before
+
+
+REGIMES = [(5, 40), (100, 40), (300, 20), (900, 20), (1500, 20), (3000, 9), (6000, 9), (12000, 5), (30000, 5), (40000, 3),
+           (40000, 600), (70000, 100), (70000, 3)]
+
+
+def everything(gpu, g, K, N, ld, top=4):
+    """One call of each entry point on a set of buffers; returns what they wrote."""
+    p = {k: v if isinstance(v, int) else v.data_ptr() for k, v in g.items()}
+    gpu.token_logprobs(p["logp"], p["ent"], p["stats"], p["sc"], p["x"], p["labels"], K, N, ld)
+    res = [to_host(g[k]).copy() for k in ("logp", "ent", "stats")]
+    d = g["d"]
+
+    def done():
+        gpu.synchronize()
+        res.append(take(d, N, K, ld) if g["off"] == 0 else to_host(d).reshape(-1)[g["off"]:g["off"] + N * ld].reshape(N, ld)[:, :K].astype(np.float64))
+        d.fill_(float(SENTINEL))
+
+    dp_ = p["d"] + 4 * g["off"]
+    gpu.token_logprobs_bwd(dp_, p["up"], p["x"], p["labels"], p["stats"], K, N, ld, ld)
+    done()
+    for e in (0.0, 0.02):
+        gpu.policy_loss(p["sums"], None, dp_, p["sc"], p["x"], p["labels"], p["old"], p["old"], p["up"], p["w"], K, N, ld, ld,
+                        0.2, 0.2, 0.1, e)
+        done()
+        res.append(to_host(g["sums"]).copy())
+    cb = (C.c_int * 3)(0, N // 3, N)
+    gpu.preference_loss(p["sums"], p["rew"], p["logp"], p["stats"], dp_, p["sc"], p["x"], p["labels"], p["old"], cb, 1, K, ld,
+                        ld, 0, 0.1, 0.0, 0, 1.0)
+    done()
+    res += [to_host(g["sums"])[:1].copy(), to_host(g["rew"]).copy()]
+    for z in (None, p["lse"]):
+        gpu.distill_topk(p["sums"], None, dp_, p["sc"], p["x"], p["t"], p["ids"], z, p["w"], K, top, N, ld, ld, top, 1.5)
+        done()
+        res.append(to_host(g["sums"])[:1].copy())
+    return res
+
+
+def buffers(K, N, ld, off, labels, seed=1, top=4):
+    r = np.random.default_rng(seed)
+    flat = np.full(N * ld + off, np.nan, F)
+    x = r.normal(0, 2, (N, K)).astype(F)
+    flat[off:].reshape(N, ld)[:, :K] = x
+    t, ids, lse, w = teacher_inputs(K, N, top, 3, 1.5, True)
+    lse[~np.isfinite(lse)] = 5.0
+    base = to_dev(flat)
+    g = dict(base=base, labels=to_dev(labels), up=to_dev(r.normal(0, 1, N).astype(F)), old=to_dev(np.full(N, -3.0, F)),
+             w=to_dev(np.abs(r.normal(0, 1, N)).astype(F)), t=to_dev(np.nan_to_num(t).reshape(-1)), ids=to_dev(ids.reshape(-1)),
+             lse=to_dev(lse), sc=scratch(N, top), logp=dev_empty(N), ent=dev_empty(N), stats=dev_empty(2 * N),
+             sums=dev_empty(4), rew=dev_empty(2), d=to_dev(np.full(N * ld + off, SENTINEL, F)), off=off)
+    g["x"] = base.data_ptr() + 4 * off
+    return g, x
+
+
+@pytest.mark.parametrize("K,N", REGIMES)
+def test_any_alignment_and_the_same_bits_again(gpu, K, N):
+    """Buffers that begin at any multiple of 4 bytes hold the same numbers to rounding, and a call
+    repeated gives the same bits."""
+    print(f"alignment K {K} N {N}", flush=True)
+    labels = np.random.default_rng(K).integers(-1, K, N).astype(np.int32)
+    labels[0], labels[-1] = 0, K - 1
+    first = None
+    for off in (0, 1, 2, 3):
+        for ld in (K, K + 2):
+            g, x = buffers(K, N, ld, off, labels)
+            got = everything(gpu, g, K, N, ld)
+            if (off, ld) in ((0, K), (3, K + 2)):
+                for a, b in zip(got, everything(gpu, g, K, N, ld)):
+                    assert np.array_equal(a, b, equal_nan=True)
+            tail = to_host(g["d"])
+            assert (tail == SENTINEL).all()
+            if first is None:
+                first = got
+                want = ref.logprobs(x, labels)[0]
+                same(got[0], want, D(K) * U + 2 * U * np.abs(want), "logp")
+                continue
+            for i, (a, b) in enumerate(zip(got, first)):
+                a, b = a.astype(np.float64), b.astype(np.float64)
+                scale = np.max(np.abs(b)) + 1.0
+                assert np.max(np.abs(a - b)) <= 64 * D(K) * U * scale, (i, off, ld)
+
+
+@pytest.mark.parametrize("K,N", REGIMES)
+def test_nothing_scored(gpu, K, N):
+    """All prompt: every loss but the pairs' is 0, every gradient is 0, nothing is NaN."""
+    labels = np.full(N, -1, np.int32)
+    labels[::2] = K
+    g, _ = buffers(K, N, K, 0, labels)
+    import torch
+    g["base"].fill_(float("nan"))
+    g["old"].fill_(float("nan"))
+    g["w"].fill_(0.0)
+    for r, want in zip(everything(gpu, g, K, N, K), [0] * 9 + [np.log(2.0)] + [0] * 5):
+        if want:
+            assert np.abs(r - want).max() <= 4 * U
+        else:
+            assert not r.any()
+    assert torch.isnan(g["base"]).all()
