@@ -834,8 +834,10 @@ constexpr size_t kMaxLds = size_t(150) << 10;   // of 160 KB, beside what the ke
 inline bool token_in_chunks(int K, int N, bool gradient) {
     // A few long columns occupy as many CUs: 1 x 262144 values 25 -> 7, gradient 41 -> 14; 64 x 131072
     // 15 -> 8.5 and 25 -> 19.  With more columns the second read of the gradient decides: 128 x 262144 gradient
-    // 56 in one piece, 63 in chunks; values 28 and 21, 256 x 262144 36 and 34.
-    return K > 2 * kMaxResident && static_cast<long long>(N) * (gradient ? 4 : 2) <= num_cus();
+    // 56 in one piece, 63 in chunks; values 28 and 21, 256 x 262144 36 and 34.  Below K = 45056 one workgroup is
+    // through before the further launches are (1 x 32000 values 6.2, 7.9 in chunks, gradient 8.7, 11.5; 1 x 50000
+    // 8.5, 7.7 and 11.4, 11.4, with the teacher's rest 14.9, 12.7).
+    return K > 11 * kChunk && static_cast<long long>(N) * (gradient ? 4 : 2) <= num_cus();
 }
 template <class Head>
 int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch, float* d, const float* x, int K, int N,
