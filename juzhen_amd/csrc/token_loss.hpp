@@ -507,7 +507,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     }
     if (team.rank < span.odd) out[span.single(team.rank)] = value(last);
     if constexpr (STREAM) {
-        constexpr int kQuads = 8, kStep = kQuads * G;
+        constexpr int kQuads = NV % 8 == 0 ? 8 : 4, kStep = kQuads * G;   // whole steps to a tile
         for (int base = (span.quads - 1) / kStep * kStep; base >= kTile; base -= kStep) {
             const Tile<G, kQuads, true> tile(team.rank, base, span.quads);
             Quad x[kQuads];
@@ -851,26 +851,33 @@ int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch,
     if (K <= kMaxTeam) return launch_token_teams<Head, 64, 16>(head, sums, d, x, K, N, ld, ldd);
     if (token_in_chunks(K, N, Head::kWrites) || head.team_bytes(K) > kMaxLds)
         return launch_token_chunks(head, sums, scratch, d, x, K, N, ld, ldd);
-    if (K <= 8192) return launch_token_columns<Head, 256, 8, 256, false>(head, sums, d, x, K, N, ld, ldd);
     if constexpr (!Head::kWrites) {
         // Values alone need no column kept; small tiles waste least of their last round: K = 24000 61 (512 x 16
         // quads in one tile: 68), 131072 65 (1024 x 24 quads: 90).
-        if (K <= 2 * 8192) return launch_token_columns<Head, 256, 4, 256, true>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 8192) return launch_token_columns<Head, 256, 8, 256, false>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 16384) return launch_token_columns<Head, 256, 4, 256, true>(head, sums, d, x, K, N, ld, ldd);
         return launch_token_columns<Head, 512, 4, 512, true>(head, sums, d, x, K, N, ld, ldd);
+    } else if (N > 2 * num_cus()) {
+        // Half of the column kept, so that several workgroups on a CU overlap their loads and stores (policy /
+        // distillation; in brackets: all of it kept by 256 x 8, 256 x 16, 512 x 16, 1024 x 16 quads): K = 5000
+        // 109 / 123 (118 / 134), 12000 150 / 172 (165 / 188), 16000 153 / 176 (162 / 187), 24000 154 / 174
+        // (165 / 187), 48000 157 / 181 (177 / 203), 64000 169 / 192 (169 / 194), the rest of the teacher's mass
+        // at 48000 188 (237); 32000 161 / 183 either way.
+        if (K <= 8192) return launch_token_columns<Head, 256, 4, 256, true>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 16384) return launch_token_columns<Head, 512, 4, 512, true>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 28672) return launch_token_columns<Head, 512, 8, 512, true>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= kMaxResident) return launch_token_columns<Head, 512, 16, 512, false>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 2 * kMaxResident) return launch_token_columns<Head, 512, 16, 512, true>(head, sums, d, x, K, N, ld, ldd);
     } else {
+        // No second workgroup to overlap with: one read (256 x 64000 23, half of it read again 25).
+        if (K <= 8192) return launch_token_columns<Head, 256, 8, 256, false>(head, sums, d, x, K, N, ld, ldd);
         if (K <= 16384) return launch_token_columns<Head, 256, 16, 256, false>(head, sums, d, x, K, N, ld, ldd);
         if (K <= kMaxResident) return launch_token_columns<Head, 512, 16, 512, false>(head, sums, d, x, K, N, ld, ldd);
-        if (K <= 2 * kMaxResident) {
-            // Half of the column kept and two workgroups on a CU, whose loads and stores overlap: K = 48000 157
-            // (one workgroup that keeps all of it: 177), 64000 170 (169), with the teacher's rest 187 (237).  Where
-            // there is no second workgroup, the one: 256 x 64000 23 (25).
-            if (N > 2 * num_cus()) return launch_token_columns<Head, 512, 16, 512, true>(head, sums, d, x, K, N, ld, ldd);
-            return launch_token_columns<Head, 1024, 16, 1024, false>(head, sums, d, x, K, N, ld, ldd);
-        }
-        // K = 98000 174 (512 threads: 197; 24 quads: 183), 262144 195 (215; 191), rest 230 (239; 248); chunks read
-        // twice over several launches 280.
-        return launch_token_columns<Head, 1024, 16, 1024, true>(head, sums, d, x, K, N, ld, ldd);
+        if (K <= 2 * kMaxResident) return launch_token_columns<Head, 1024, 16, 1024, false>(head, sums, d, x, K, N, ld, ldd);
     }
+    // K = 98000 174 (512 threads: 197; 24 quads: 183), 262144 195 (215; 191), rest 230 (239; 248); chunks read
+    // twice over several launches 280.
+    if constexpr (Head::kWrites) return launch_token_columns<Head, 1024, 16, 1024, true>(head, sums, d, x, K, N, ld, ldd);
 }
 
 // The arguments every entry point of this family checks alike.

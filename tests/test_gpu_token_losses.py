@@ -24,7 +24,9 @@ SHAPES = [(1, 1, 0, 0), (2, 3, 0, 0), (3, 70, 1, 0), (13, 33, 0, 0), (16, 4, 0, 
           (65, 129, 3, 1), (128, 9, 0, 0), (130, 64, 0, 0), (256, 96, 0, 0), (257, 31, 1, 0), (512, 5, 0, 0),
           (1000, 40, 0, 0), (1024, 16, 0, 8), (1025, 7, 0, 0), (4096, 6, 0, 0), (4099, 300, 2, 0), (8200, 5, 0, 0),
           (16385, 4, 0, 3), (32000, 300, 0, 0), (32771, 3, 0, 0), (50001, 2, 0, 0), (65537, 260, 0, 0), (98309, 2, 1, 0),
-          (131072, 3, 0, 0), (131077, 2, 0, 0), (200003, 5, 0, 1)]
+          (131072, 3, 0, 0), (131077, 2, 0, 0), (200003, 5, 0, 1),
+          # enough columns for several workgroups on a CU
+          (5001, 530, 0, 0), (12000, 520, 1, 1), (20001, 515, 0, 2), (45000, 513, 0, 0)]
 
 
 def D(K):
