@@ -449,7 +449,7 @@ int jzhip_softmax_xent_dense(float* loss_out, float* dlogits, const float* logit
  *     quantities (log-probability, ratio, divergence) and the sums over tokens, all in a fixed
  *     order: the same call on the same buffers gives the same bits, and values are the same
  *     with dlogits as without.  (Another address modulo 16 bytes groups a column differently.)
- *   - K up to 2^28, N and ld as int allows; offsets are 64 bits wide.
+ *   - K up to 2^28, N up to 2^25, K * N up to 2^36, ld as int allows; offsets are 64 bits wide.
  *   - scratch: caller-provided, 16-byte aligned, jzhip_token_scratch_floats(N, top) =
  *     (8 + top) * N + 2^20 floats (top: 0 but for jzhip_distill_topk; for
  *     jzhip_preference_loss N is the number of tokens).  Nothing in it outlives a call, and no

@@ -58,6 +58,7 @@ struct BwdArgs {
     int K, N;
     size_t ld, ldd;
     ExpScale scale;
+    int first = 0;   // column of the launch's first workgroup
 };
 template <int G, int NV, bool NT>
 __device__ __forceinline__ void bwd_span(const BwdArgs& a, const Team<G>& team, size_t col, int base) {
@@ -121,10 +122,10 @@ __global__ __launch_bounds__(G > kWave ? G : kBwdBlock) void logprob_bwd_kernel(
     __shared__ double slots[kBlock / kWave];
     if (total.out && blockIdx.x == 0) fold_parts<kBlock>(total.out, total.losses, total.pairs, total.scale, slots);
     const Team<G> team{static_cast<int>(threadIdx.x % G)};
-    const int col = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
-    if (kTeams > 1 && col >= a.N) return;
-    const int base = kTeams > 1 ? 0 : static_cast<int>(blockIdx.x - col * chunks.d) * G;
-    bwd_span<G, (kTeams > 1 ? kGroupQuads : 1), NT>(a, team, col, base);
+    const int n = kTeams > 1 ? static_cast<int>(blockIdx.x * kTeams + threadIdx.x / G) : static_cast<int>(fdiv(blockIdx.x, chunks));
+    if (kTeams > 1 && n >= a.N) return;
+    const int base = kTeams > 1 ? 0 : static_cast<int>(blockIdx.x - n * chunks.d) * G;
+    bwd_span<G, (kTeams > 1 ? kGroupQuads : 1), NT>(a, team, static_cast<size_t>(a.first) + n, base);
 }
 
 template <bool ENTROPY, bool EXACT>
@@ -135,15 +136,23 @@ int logprobs(float* logp, float* entropy, float* stats, double* exact, float* sc
 }
 
 template <int G>
-int launch_bwd(const BwdArgs& a, const PairTotal& total) {
+int launch_bwd(BwdArgs a, PairTotal total) {
     constexpr int kBlock = G > kWave ? G : kBwdBlock, kTeams = kBlock / G;
     const int chunks = kTeams > 1 ? 1 : (a.K / 4 + G - 1) / G;
-    const size_t blocks = (static_cast<size_t>(a.N) * chunks + kTeams - 1) / kTeams;
-    if (blocks > 0x7fffffffull) return -1;
     const bool nt = streams_past_cache(static_cast<size_t>(a.K) * a.N * 2 * sizeof(float));
     auto kernel = nt ? logprob_bwd_kernel<G, true> : logprob_bwd_kernel<G, false>;
-    kernel<<<static_cast<unsigned>(blocks), kBlock, 0, stream()>>>(a, total, make_fastdiv(chunks));
-    return launch_rc();
+    // A thread per quad: what a launch may have (2^32 threads) is 2^34 logits.  Columns beyond go in
+    // launches of their own.  (Columns of small teams are few enough: kMaxTokens.)
+    const int most = kTeams > 1 ? a.N : static_cast<int>(kMaxThreads / kBlock) / chunks;
+    for (; a.first < a.N; a.first += most) {
+        const int n = a.N - a.first < most ? a.N - a.first : most;
+        const unsigned blocks = static_cast<unsigned>((static_cast<size_t>(n) * chunks + kTeams - 1) / kTeams);
+        kernel<<<blocks, kBlock, 0, stream()>>>(a, total, make_fastdiv(chunks));
+        const int rc = launch_rc();
+        if (rc) return rc;
+        total.out = nullptr;
+    }
+    return 0;
 }
 int logprobs_bwd(const BwdArgs& a, const PairTotal& total) {
     if (a.K <= 64) return launch_bwd<4>(a, total);

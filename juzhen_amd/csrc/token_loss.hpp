@@ -600,6 +600,8 @@ constexpr int kMaxChunks = (1 << 19) * 4 / static_cast<int>(sizeof(ChunkSums));
 constexpr int kMaxColumns = (1 << 19) * 4 / static_cast<int>(sizeof(ColumnCoef));
 constexpr size_t kScratchFixed = size_t(1) << 20;
 constexpr int kMaxK = kChunk * kMaxChunks;
+constexpr int kMaxTokens = 1 << 25;
+constexpr unsigned long long kMaxLogits = 1ull << 36, kMaxThreads = (1ull << 32) - 1;   // of a launch
 static_assert(sizeof(ChunkSums) == 32 && sizeof(ColumnCoef) == 32, "scratch layout");
 
 template <class Head>
@@ -880,9 +882,12 @@ int launch_token_kernel(const Head& head, const TokenSums& sums, float* scratch,
     if constexpr (Head::kWrites) return launch_token_columns<Head, 1024, 16, 1024, true>(head, sums, d, x, K, N, ld, ldd);
 }
 
-// The arguments every entry point of this family checks alike.
+// The arguments every entry point of this family checks alike.  With at most 64 threads to a column of up
+// to 4096 logits, 256 to 8192, 512 to 65536 and 1024 beyond, kMaxTokens columns and kMaxLogits logits keep every
+// launch below kMaxThreads.
 inline bool token_args_ok(const float* x, const float* d, const float* scratch, int K, int N, int ld, int ldd) {
     if (K <= 0 || K > kMaxK || N <= 0 || ld < K || !x || !aligned16(scratch)) return false;
+    if (N > kMaxTokens || static_cast<unsigned long long>(K) * N > kMaxLogits) return false;
     if (d && (ldd < K || (d == x && ldd != ld))) return false;
     return true;
 }

@@ -119,6 +119,30 @@ def test_far_offsets_and_long_columns(gpu, K, N, ld, live):
         assert abs(to_host(one)[0] - loss) <= D(K) * U + 4 * U * (1 + loss)
 
 
+def test_gradient_over_several_launches(gpu):
+    """2^23 + 300 columns of 1025 logits (34 GB), in place: with 512 threads to a column, more threads than a
+    launch may have.  All logits 0, sums as of a column of 1025 ones: -g/1025, and g - g/1025 at the label, off by
+    the roundings of the sum's quotient, of the exponential (1 ulp) and of the products (4 U |g|)."""
+    import torch
+    K, N = 1025, (1 << 23) + 300
+    print(f"far gradient K {K} N {N}", flush=True)
+    x = torch.zeros(N, K, dtype=torch.float32, device="cuda")
+    n = torch.arange(N, device="cuda")
+    labels = (n % K).to(torch.int32)
+    labels[5::1000] = -1
+    g = ((n % 7) + 1).to(torch.float32)
+    stats = torch.cat([torch.zeros(N, device="cuda"), torch.full((N,), float(K), device="cuda")])
+    torch.cuda.synchronize()
+    gpu.token_logprobs_bwd(dptr(x), dptr(g), dptr(x), dptr(labels), dptr(stats), K, N, K, K)
+    to_host(g[:1])   # waits
+    for at in range(0, N, 1 << 20):
+        rows, lab, up = x[at:at + (1 << 20)], labels[at:at + (1 << 20)].long(), g[at:at + (1 << 20)]
+        up = torch.where(lab >= 0, up, torch.zeros_like(up))
+        rows[torch.arange(len(lab), device="cuda"), lab.clamp(min=0)] -= up
+        off = torch.maximum((rows.amax(1) + up / K).abs(), (rows.amin(1) + up / K).abs())
+        assert bool((off <= 4 * U * up).all()), at
+
+
 def to_keep(a):
     import util
     t = to_dev(a)

@@ -83,6 +83,17 @@ def test_distill_refuses(lib):
         assert lib.jzhip_distill_topk(*a) == -1, (at, bad)
 
 
+# more columns, or more logits, than a launch has threads for
+@pytest.mark.parametrize("K,N", [(8, (1 << 25) + 1), (8, (1 << 31) - 1), (4097, 1 << 24), (1 << 28, 257)])
+def test_sizes_beyond_a_launch(lib, K, N):
+    begin = (INT * 3)(0, 1, N)
+    assert lib.jzhip_token_logprobs(P, None, None, P, P, P, K, N, K) == -1
+    assert lib.jzhip_token_logprobs_bwd(P, P, Q, P, P, K, N, K, K) == -1
+    assert lib.jzhip_policy_loss(P, P, Q, P, P, P, P, P, P, P, K, N, K, K, 0.2, 0.2, 0.1, 0.0) == -1
+    assert lib.jzhip_preference_loss(P, P, P, P, Q, P, P, P, None, begin, 1, K, K, K, 0, 0.1, 0.0, 0, 1.0) == -1
+    assert lib.jzhip_distill_topk(P, None, Q, P, P, P, P, None, None, K, 2, N, K, K, 2, 1.0) == -1
+
+
 def _slope(f, x, v, h=1e-5):
     return (f(x + h * v) - f(x - h * v)) / (2 * h)
 
