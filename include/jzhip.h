@@ -505,7 +505,8 @@ int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, float* s
  *   teacher_lse == NULL: lse over the column's entries,
  *       l = T^2 * sum_j q_j log(q_j / p(id_j))
  *   teacher_lse (N): log sum exp(teacher / T) over the teacher's whole vocabulary; what the
- *       entries leave, max(0, 1 - sum q_j), is one more class against the p of everything else.
+ *       entries leave, max(0, 1 - sum q_j), is one more class against the p of everything else
+ *       (however far those logits lie below the entries; infinite where all of them are masked).
  * loss_out[0] = sum_n w_n l_n (weight NULL: all 1), token_loss (N, may be NULL) = l_n, dlogits
  * the gradient of loss_out.  A column without entries (or, with teacher_lse NULL, of entries
  * of -inf only) is not scored.  temperature in [1e-3, 1e3]. */

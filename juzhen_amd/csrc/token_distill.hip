@@ -7,9 +7,16 @@
 //   P_j = p_(id_j),  P_rest = sum of the p_i that are no entry
 //   L   = w * T^2 * sum_g q_g log(q_g / P_g)
 //   d_i = w * T * (Q p_i - q_g(i) p_i / P_g(i)),  Q = sum_g q_g
-// P_rest is summed over its own members: 1 - sum P_j would lose it where the entries cover
-// nearly all of the student's mass, and the gradient divides by it.
+// P_rest is summed over its own members, relative to the largest of them: 1 - sum P_j, and a sum
+// relative to the column's maximum, would lose it where the student gives the entries nearly all
+// of its mass (logits 87 T above the others: exp underflows), and the gradient divides by it.  The
+// sweep leaves the entries out, and finish() adds them in 64 bits: with m', s' of the rest,
+//   M = max(m', entries),  S = s' exp((m' - M)/T) + sum_j exp((x_j - M)/T)
+//   log P_rest = (m' - M)/T + log s' - log S
+//   d_i = e'_i * w T (Q exp((m' - M)/T)/S - q_rest/s'),  e'_i = exp((x_i - m')/T)   (i in the rest)
 #include "token_loss.hpp"
+
+#include <cfloat>
 
 namespace jz {
 namespace {
@@ -32,7 +39,9 @@ struct DistillHead {
     static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true, kExact = false;
     struct Early {
         float w;
-        double Q;   // sum of the q_j, from the prologue
+        // from the prologue: REST: maximum and sum of the student's entries; sum of the q_j
+        float m;
+        double s, Q;
     };
     ExpScale scale;
     const float* teacher;
@@ -61,7 +70,7 @@ struct DistillHead {
     }
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
-    __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, 0.0}; }
+    __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, -INFINITY, 0.0, 0.0}; }
     __device__ void write(size_t col, float each, float loss) const {
         if (token_loss) token_loss[col] = each;
         part[col] = loss;
@@ -83,6 +92,7 @@ struct DistillHead {
             e.lq[j] = static_cast<double>(t);
             if (!is) continue;
             e.x[j] = x[id];
+            if (REST) early.m = fmaxf(early.m, e.x[j]);
             big = fmaxf(big, t);
             if (all) {
                 const unsigned bit = 1u << (id & 31);
@@ -111,8 +121,11 @@ struct DistillHead {
         double Q = 0.0;
         if constexpr (REST) {
             const double norm = static_cast<double>(lse[col]);
+            early.m = lead.lanes(early.m, LargerOp{});
+            const double shift = early.m == -INFINITY ? 0.0 : static_cast<double>(early.m);
             for (int j = lead.rank; j < top; j += T::kSize) {
                 if (e.id[j] < 0) continue;
+                early.s += exp64((static_cast<double>(e.x[j]) - shift) * over);
                 const double u = e.lq[j] * over - norm, q = exp64(u);
                 e.lq[j] = u;
                 e.q[j] = static_cast<float>(q);
@@ -120,6 +133,7 @@ struct DistillHead {
                 some = 1.f;
             }
             Q = lead.lanes(Q, AddOp{});
+            early.s = lead.lanes(early.s, AddOp{});
         } else {
             big = lead.lanes(big, LargerOp{});
             double z = 0.0;
@@ -143,46 +157,59 @@ struct DistillHead {
         early.Q = Q;
         return lead.lanes(some, LargerOp{}) != 0.f;
     }
-    // f.g: Q*T*w/s, f.x: T*w
-    __device__ float entry_gradient(const Entries& e, int j, float m, const Grad& f) const {
-        return exp_shifted(e.x[j] - m, scale) * f.g - f.x * e.q[j];
+    // f.g: Q*T*w/s, f.x: T*w, f.b: the maximum of the whole column
+    __device__ float entry_gradient(const Entries& e, int j, const Grad& f) const {
+        return exp_shifted(e.x[j] - f.b, scale) * f.g - f.x * e.q[j];
     }
     template <class T>
     __device__ Grad finish(const T& lead, char* own, const Early& early, size_t col, const ColumnSums& c) const {
         const Entries e(own, top);
-        const double T_ = static_cast<double>(temperature), over = 1.0 / T_, logs = log64(c.s);
+        const double T_ = static_cast<double>(temperature), over = 1.0 / T_;
         const double w = static_cast<double>(early.w);
+        float big = c.m;
+        double s = c.s, below = 1.0;   // below: what the rest's exponentials are to those relative to `big`
+        if constexpr (REST) {
+            big = fmaxf(c.m, early.m);
+            const bool higher = c.m >= early.m;
+            const double f = exp64(-fabs((static_cast<double>(c.m) - static_cast<double>(early.m)) * over));
+            below = c.m == -INFINITY ? 0.0 : higher ? 1.0 : f;
+            s = c.s * below + early.s * (early.m == -INFINITY ? 0.0 : higher && c.m != early.m ? f : 1.0);
+        }
+        const double logs = log64(s);
         double Q = early.Q, each = 0.0;
         for (int j = lead.rank; j < top; j += T::kSize) {
             // an entry of no mass adds nothing, whatever the student gives it; a NaN stays one
             if (e.id[j] < 0 || e.q[j] == 0.f) continue;
             each += static_cast<double>(e.q[j]) *
-                    (e.lq[j] - ((static_cast<double>(e.x[j]) - static_cast<double>(c.m)) * over - logs));
+                    (e.lq[j] - ((static_cast<double>(e.x[j]) - static_cast<double>(big)) * over - logs));
         }
         each = lead.lanes(each, AddOp{});
-        const double inv = 1.0 / c.s;
+        const double inv = 1.0 / s;
         double out = 0.0;   // what the rest subtracts
         if constexpr (REST) {
             double r = 1.0 - Q;
             r = r < 0.0 ? 0.0 : r;
-            if (r != 0.0) each += r * (log64(r) - log64(c.rest * inv));
+            // the type's lowest value beside larger logits is a mask
+            const double rest = c.m == -FLT_MAX && big > c.m ? 0.0 : c.s;
+            if (r != 0.0)
+                each += r * (log64(r) - ((static_cast<double>(c.m) - static_cast<double>(big)) * over + log64(rest) - logs));
             Q += r;
-            out = c.rest > 0.0 ? r / c.rest : Q * inv;
+            if (rest > 0.0) out = r / rest;
         }
         each *= T_ * T_;
         if (lead.rank == 0) write(col, static_cast<float>(each), static_cast<float>(w * each));
-        const Grad f{static_cast<float>(T_ * w * (Q * inv - out)), 0.f, static_cast<float>(T_ * w * (Q * inv)),
+        const Grad f{static_cast<float>(T_ * w * (Q * below * inv - out)), big, static_cast<float>(T_ * w * (Q * inv)),
                      static_cast<float>(T_ * w)};
         if (chunked)
             for (int j = lead.rank; j < top; j += T::kSize)
-                if (e.id[j] >= 0) picked[col * top + j] = entry_gradient(e, j, c.m, f);
+                if (e.id[j] >= 0) picked[col * top + j] = entry_gradient(e, j, f);
         return f;
     }
     template <class T>
-    __device__ void correct(const T& lead, char* own, size_t, float m, const Grad& f, float* out) const {
+    __device__ void correct(const T& lead, char* own, size_t, float, const Grad& f, float* out) const {
         const Entries e(own, top);
         for (int j = lead.rank; j < top; j += T::kSize)
-            if (e.id[j] >= 0) out[e.id[j]] = entry_gradient(e, j, m, f);
+            if (e.id[j] >= 0) out[e.id[j]] = entry_gradient(e, j, f);
     }
     // The entries among the logits [begin, begin + len), whose gradients `picked` holds.
     template <class T>

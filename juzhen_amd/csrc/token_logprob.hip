@@ -295,11 +295,11 @@ __global__ __launch_bounds__(kSmallBlock, 4) void preference_small_kernel(Logpro
     for (int r = 0; r < kSmallRounds; ++r) {
         const int n = slot + r * kTeams;
         if (n >= a.N) continue;
-        c[r] = ColumnSums{-INFINITY, 0.0, 0.0, 0.0};
+        c[r] = ColumnSums{-INFINITY, 0.0, 0.0};
         const Group g = take_group<Head>(v[r], head.scale, [](int) { return 0u; });
         group[r] = g.m;
         add_group<Head>(c[r], g, head.scale);
-        if (team.rank < span[r].odd) add_group<Head>(c[r], take_one<Head>(last[r], false), head.scale);
+        if (team.rank < span[r].odd) add_group<Head>(c[r], take_one<Head>(last[r]), head.scale);
         scale_sums<Head>(c[r], team.reduce(c[r].m, LargerOp{}, static_cast<float*>(nullptr)), head.scale);
         c[r].s = team.reduce(c[r].s, AddOp{}, static_cast<double*>(nullptr));
         live[r] = live[r] && !(c[r].m == -INFINITY && c[r].s == c[r].s);

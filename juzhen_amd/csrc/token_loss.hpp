@@ -180,14 +180,17 @@ struct Team {
     __device__ __forceinline__ Team<kLanes> lead() const { return Team<kLanes>{rank}; }
 };
 
-// What one sweep over a column leaves: its maximum, the sum of e_i, of e_i*t_i (heads
-// that ask for the entropy) and of the e_i that are none of the teacher's entries
-// (heads that ask for the rest).
+// What one sweep over a column leaves: its maximum, the sum of e_i and of e_i*t_i (heads
+// that ask for the entropy).  Heads that ask for the rest (kRest) sweep over the logits that are
+// none of the teacher's entries, with a maximum of their own, and add the entries themselves.
 struct ColumnSums {
     float m;
-    double s, et, rest;
+    double s, et;
 };
-// d_i = e_i * (a + b*t_i); g is added at the label, whose logit is x.
+// Something is left but masked logits: a number, or a NaN.
+__device__ __forceinline__ bool unmasked(float m, double s) { return !(m == -INFINITY && s == s); }
+// d_i = e_i * (a + b*t_i); g is added at the label, whose logit is x.  (A head without the entropy
+// has b for itself.)
 struct Grad {
     float a, b, g, x;
 };
@@ -250,19 +253,26 @@ __device__ __forceinline__ float quad_max(const Quad& v) { return fmaxf(fmaxf(v.
 // only a factor exp(m_group - m) once that is known.
 constexpr int kGroupQuads = 4;
 struct Group {
-    float m, s, ones, et, rest;   // exact heads: s of the exponentials below 1, ones: how many are 1
+    float m, s, ones, et;   // exact heads: s of the exponentials below 1, ones: how many are 1
 };
 // x: the group's logits; without the entropy they become e_i relative to the group.  known(k): the
-// teacher's entries among quad k.
+// teacher's entries among quad k, which do not count.
 template <class Head, class Known>
 __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpScale& scale, Known known) {
-    Group g{-INFINITY, 0.f, 0.f, 0.f, 0.f};
+    Group g{-INFINITY, 0.f, 0.f, 0.f};
     float top[kGroupQuads];
 #pragma unroll
-    for (int k = 0; k < kGroupQuads; ++k) top[k] = quad_max(x[k]);
+    for (int k = 0; k < kGroupQuads; ++k) {
+        if constexpr (Head::kRest) {
+            const unsigned b = known(k);
+            x[k] = Quad{b & 1u ? -INFINITY : x[k].x, b & 2u ? -INFINITY : x[k].y, b & 4u ? -INFINITY : x[k].z,
+                        b & 8u ? -INFINITY : x[k].w};
+        }
+        top[k] = quad_max(x[k]);
+    }
     g.m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     const float shift = g.m == -INFINITY ? 0.f : g.m;   // nothing but -inf: sums of 0; a NaN still shows
-    float s[kGroupQuads], all[kGroupQuads], et[kGroupQuads], rest[kGroupQuads];
+    float s[kGroupQuads], all[kGroupQuads], et[kGroupQuads];
 #pragma unroll
     for (int k = 0; k < kGroupQuads; ++k) {
         const float t0 = x[k].x - shift, t1 = x[k].y - shift, t2 = x[k].z - shift, t3 = x[k].w - shift;
@@ -276,10 +286,6 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
             et[k] = (e0 * fmaxf(t0, -200.f) + e1 * fmaxf(t1, -200.f)) + (e2 * fmaxf(t2, -200.f) + e3 * fmaxf(t3, -200.f));
         else
             x[k] = Quad{e0, e1, e2, e3};
-        if constexpr (Head::kRest) {
-            const unsigned b = known(k);
-            rest[k] = ((b & 1u ? 0.f : e0) + (b & 2u ? 0.f : e1)) + ((b & 4u ? 0.f : e2) + (b & 8u ? 0.f : e3));
-        }
     }
     g.s = (all[0] + all[1]) + (all[2] + all[3]);
     if constexpr (Head::kExact) {
@@ -288,7 +294,6 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
         g.s = below;
     }
     if constexpr (Head::kEntropy) g.et = (et[0] + et[1]) + (et[2] + et[3]);
-    if constexpr (Head::kRest) g.rest = (rest[0] + rest[1]) + (rest[2] + rest[3]);
     return g;
 }
 // Joins sums relative to two maxima (the shift of sums of nothing but -inf is 0: they are 0, or
@@ -299,26 +304,24 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
     const float t = c.m - m;
     const double f = t == 0.f ? 1.0 : static_cast<double>(exp_shifted(t, scale)) * (1.0 + kExpShort);
     if constexpr (Head::kEntropy) c.et = (c.et + c.s * static_cast<double>(fmaxf(t, -200.f))) * f;
-    if constexpr (Head::kRest) c.rest *= f;
     c.s *= f;
     c.m = m;
 }
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
     ColumnSums more{g.m, (Head::kExact ? static_cast<double>(g.ones) : 0.0) + static_cast<double>(g.s) * (1.0 + kExpShort),
-                    static_cast<double>(g.et), static_cast<double>(g.rest)};
+                    static_cast<double>(g.et)};
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
     scale_sums<Head>(more, m, scale);
     c.s += more.s;
     if constexpr (Head::kEntropy) c.et += more.et;
-    if constexpr (Head::kRest) c.rest += more.rest;
 }
 // of a single logit
 template <class Head>
-__device__ __forceinline__ Group take_one(float x, bool known) {
+__device__ __forceinline__ Group take_one(float x) {
     const float e = x == -INFINITY ? 0.f : x - x + 1.f;   // exp of its shift from itself; a NaN or +inf shows
-    return Group{x, Head::kExact ? 0.f : e, e, 0.f, known ? 0.f : e};
+    return Group{x, Head::kExact ? 0.f : e, e, 0.f};
 }
 
 // The compiler would interleave the independent work of an unrolled loop and spill what it
@@ -357,7 +360,7 @@ struct ColumnShared {
     float max[Team<G>::kWaves];
     double s[Team<G>::kWaves], other[Team<G>::kWaves];
     Grad grad;
-    int live;
+    int live;   // 2: also if nothing but the teacher's entries is left
 };
 
 // One column by one team: NV quads per thread in registers, what is beyond them (STREAM) in tiles
@@ -378,7 +381,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     Quad v[kGroups][kGroupQuads];
     float group_max[kGroups];
     float last = -INFINITY;
-    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
+    ColumnSums c{-INFINITY, 0.0, 0.0};
     typename Head::Early early{};
     if (live) {
         const unsigned* bits = nullptr;
@@ -401,7 +404,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
                 if (!team.leads()) return;
                 const bool some = head.prologue(team.lead(), own, marks, col, K, p, early);
                 if constexpr (Team<G>::kWorkgroup) {
-                    if (team.rank == 0) sh.live = some;
+                    if (team.rank == 0) sh.live = some ? 1 + unmasked(early.m, early.s) : 0;
                 } else {
                     live = some;
                 }
@@ -447,27 +450,33 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
             in_order<NV>();
         }
         if (team.rank < span.odd) {
-            bool known = false;
-            if constexpr (Head::kRest) known = known_one(bits, span.single(team.rank));
-            add_group<Head>(c, take_one<Head>(last, known), head.scale);
+            if constexpr (Head::kRest)
+                if (known_one(bits, span.single(team.rank))) last = -INFINITY;
+            add_group<Head>(c, take_one<Head>(last), head.scale);
         }
         scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
-        if constexpr (Head::kTeacher && Team<G>::kWorkgroup) live = sh.live;   // behind that barrier
-        if constexpr (Head::kEntropy || Head::kRest) {
-            double& more = Head::kEntropy ? c.et : c.rest;
-            more = team.lanes(more, AddOp{});
+        bool filled = false;   // an entry that is not masked
+        if constexpr (Head::kTeacher) {
+            filled = unmasked(early.m, early.s);
+            if constexpr (Team<G>::kWorkgroup) {   // behind that barrier
+                live = sh.live != 0;
+                filled = sh.live == 2;
+            }
+        }
+        if constexpr (Head::kEntropy) {
+            c.et = team.lanes(c.et, AddOp{});
             if constexpr (Team<G>::kWorkgroup)
-                if ((team.rank & (kWave - 1)) == 0) sh.other[team.rank / kWave] = more;
+                if ((team.rank & (kWave - 1)) == 0) sh.other[team.rank / kWave] = c.et;
             c.s = team.reduce(c.s, AddOp{}, sh.s);
             if constexpr (Team<G>::kWorkgroup) {
-                more = sh.other[0];
+                c.et = sh.other[0];
 #pragma unroll
-                for (int k = 1; k < Team<G>::kWaves; ++k) more += sh.other[k];
+                for (int k = 1; k < Team<G>::kWaves; ++k) c.et += sh.other[k];
             }
         } else {
             c.s = team.reduce(c.s, AddOp{}, sh.s);
         }
-        live = live && !(c.m == -INFINITY && c.s == c.s);   // nothing left but masked entries; NaN counts
+        live = live && (filled || unmasked(c.m, c.s));
     }
     if (!live) {
         if (team.rank == 0) head.idle(col);
@@ -486,14 +495,15 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         f = sh.grad;
     }
     float* const to = out + span.skew;
-    auto value = [&](float x) {
-        const float t = x - c.m;
+    const float shift = c.m == -INFINITY ? 0.f : c.m;   // (exponentials are 0 then, or NaN)
+    auto value = [&](float x) {   // (at an entry of the rest anything: its own gradient comes behind)
+        const float t = x - shift;
         return grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), f.a, f.b);
     };
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
         float scale = 0.f;
-        if constexpr (kKeepMax) scale = (c.m == -INFINITY ? 1.f : exp_shifted(group_max[i] - c.m, head.scale)) * f.a;
+        if constexpr (kKeepMax) scale = exp_shifted(group_max[i] - shift, head.scale) * f.a;
 #pragma unroll
         for (int k = 0; k < kGroupQuads; ++k) {
             const Quad x = v[i][k];
@@ -524,7 +534,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         }
     }
     team.sync();   // behind the sweep that wrote these elements as any other
-    if (team.leads()) head.correct(team.lead(), own, col, c.m, f, out);
+    if (team.leads()) head.correct(team.lead(), own, col, shift, f, out);
 }
 
 // *out = scale * sum of p[0 ... n) by a wave or a workgroup of BLOCK threads, in 64 bits in a fixed order.
@@ -587,8 +597,8 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
 constexpr int kChunkBlock = 256;
 constexpr int kChunk = 4 * kChunkBlock * kGroupQuads;
 struct ChunkSums {
-    double s, et, rest;
-    float m, pad;
+    double s, et;
+    float m, pad[3];
 };
 struct ColumnCoef {
     Grad f;
@@ -624,7 +634,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, Chu
         v[k] = Quad(-INFINITY);
         if (q < span.quads) v[k] = load_quad<false>(p + span.skew + 4 * q);
     }
-    const float last = team.rank < span.odd ? p[span.single(team.rank)] : -INFINITY;
+    float last = team.rank < span.odd ? p[span.single(team.rank)] : -INFINITY;
     if constexpr (Head::kRest) {
         for (int i = team.rank; i < kChunk / 32; i += G) bits[i] = 0u;
         __syncthreads();
@@ -635,22 +645,17 @@ __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, Chu
         const int q = team.rank + k * G;
         return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));
     });
-    ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
+    ColumnSums c{-INFINITY, 0.0, 0.0};
     add_group<Head>(c, g, head.scale);
     if (team.rank < span.odd) {
-        bool known = false;
-        if constexpr (Head::kRest) known = known_one(bits, span.single(team.rank));
-        add_group<Head>(c, take_one<Head>(last, known), head.scale);
+        if constexpr (Head::kRest)
+            if (known_one(bits, span.single(team.rank))) last = -INFINITY;
+        add_group<Head>(c, take_one<Head>(last), head.scale);
     }
     scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
-    double more = team.lanes(Head::kEntropy ? c.et : c.rest, AddOp{});
-    if ((team.rank & (kWave - 1)) == 0) sh.other[team.rank / kWave] = more;
+    if constexpr (Head::kEntropy) c.et = team.reduce(c.et, AddOp{}, sh.other);
     c.s = team.reduce(c.s, AddOp{}, sh.s);
-    if (team.rank == 0) {
-        more = sh.other[0];
-        for (int w = 1; w < Team<G>::kWaves; ++w) more += sh.other[w];
-        sums[blockIdx.x] = ChunkSums{c.s, Head::kEntropy ? more : 0.0, Head::kRest ? more : 0.0, c.m, 0.f};
-    }
+    if (team.rank == 0) sums[blockIdx.x] = ChunkSums{c.s, c.et, c.m, {}};
 }
 
 template <class Head>
@@ -659,7 +664,6 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
                                                                  size_t ld) {
     constexpr int G = kChunkBlock;
     __shared__ ColumnShared<G> sh;
-    __shared__ double third[Team<G>::kWaves];
     extern __shared__ __align__(16) char dynamic[];
     const Team<G> team{static_cast<int>(threadIdx.x)};
     const size_t col = col0 + blockIdx.x;
@@ -668,7 +672,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
     bool live = head.live(col, K);
     if (live) {   // for the whole workgroup
         typename Head::Early early = head.early(col, p);
-        ColumnSums c{-INFINITY, 0.0, 0.0, 0.0};
+        ColumnSums c{-INFINITY, 0.0, 0.0};
         const ChunkSums* q = sums + static_cast<size_t>(blockIdx.x) * chunks;
         for (int i = team.rank; i < chunks; i += G) c.m = fmaxf(c.m, q[i].m);
         c.m = team.reduce(c.m, LargerOp{}, sh.max);
@@ -680,17 +684,19 @@ __global__ __launch_bounds__(kChunkBlock) void token_join_kernel(Head head, Colu
             const double f = exp64(t * inv * 0.69314718055994531);
             c.s += w.s * f;
             c.et += (w.et + w.s * (t < -1e4 ? -1e4 : t)) * f;
-            c.rest += w.rest * f;
         }
         c.s = team.reduce(c.s, AddOp{}, sh.s);
         if constexpr (Head::kEntropy) c.et = team.reduce(c.et, AddOp{}, sh.other);
-        if constexpr (Head::kRest) c.rest = team.reduce(c.rest, AddOp{}, third);
         if (!team.leads()) return;
-        live = !(c.m == -INFINITY && c.s == c.s);
-        if constexpr (Head::kTeacher) live = live && head.prologue(team.lead(), dynamic, nullptr, col, K, p, early);
+        bool filled = false;
+        if constexpr (Head::kTeacher) {
+            live = head.prologue(team.lead(), dynamic, nullptr, col, K, p, early);
+            filled = unmasked(early.m, early.s);
+        }
+        live = live && (filled || unmasked(c.m, c.s));
         if (live) {
             r.f = head.finish(team.lead(), dynamic, early, col, c);
-            r.m = c.m;
+            r.m = c.m == -INFINITY ? 0.f : c.m;   // as in token_column
             r.live = 1;
             r.label = head.label(col);
         }
