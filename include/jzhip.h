@@ -488,7 +488,8 @@ int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* scratch,
  * (jzhip_token_logprobs), NULL for none; read for scored tokens only.
  *   R_s = beta * sum (log p(label) - ref_logp) over its scored tokens, divided by their number
  *   when average != 0 (0 if there is none);  h_p = R_2p - R_2p+1
- *   kind 0: l = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)   (smoothing < 0.5)
+ *   kind 0: l = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)   (smoothing < 0.5; 0: the
+ *   second term is absent, so that a rejected answer of probability 0 has loss 0)
  *   kind 1: l = max(0, 1 - h)         kind 2: l = ((h - 1/2) / beta)^2    (smoothing 0)
  * loss_out[0] = scale * sum_p l(h_p), rewards (2*pairs) = R, logp and stats as
  * jzhip_token_logprobs writes them (both needed), dlogits the gradient of loss_out.  A pair's

@@ -214,7 +214,9 @@ __device__ __forceinline__ void take_pair(const PairArgs& a, const T& team, int 
         const double z = exp64(-fabs(h)), tail = z < 1e-5 ? z - 0.5 * z * z : log64(1.0 + z);   // log(1 + z)
         const double down = (h >= 0.0 ? z : 1.0) / (1.0 + z), up = (h >= 0.0 ? 1.0 : z) / (1.0 + z);   // sigma(-h), sigma(h)
         const double sm = static_cast<double>(a.smoothing);
-        loss = (1.0 - sm) * (tail + (h >= 0.0 ? 0.0 : -h)) + sm * (tail + (h >= 0.0 ? h : 0.0));
+        // -h, h: of the terms -log sigma(h) = tail + max(-h, 0), -log sigma(-h) = tail + max(h, 0); what has
+        // no part is left out (h is infinite where a label has probability 0)
+        loss = tail + (h >= 0.0 ? (sm != 0.0 ? sm * h : 0.0) : (1.0 - sm) * -h);
         slope = -(1.0 - sm) * down + sm * up;
     } else if (a.kind == kHinge) {
         loss = h >= 1.0 ? 0.0 : 1.0 - h;
