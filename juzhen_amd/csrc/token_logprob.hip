@@ -49,7 +49,7 @@ struct LogprobHead {
 // cut into workgroups of 512 threads with one quad each, which keeps the accesses in flight
 // closest together (32000 x 4194, a quarter of the tokens unscored: 151 us, 2 quads 173; 256
 // threads with 1, 2, 4 quads 149, 158, 176, but 163 to 151 at 50001 x 2684).
-constexpr int kBwdBlock = 256, kBwdLong = 512;
+constexpr int kBwdBlock = 256, kBwdLong = 512, kBwdTeams = 1024;   // kBwdTeams: up to so many logits a wave or less
 struct BwdArgs {
     float* d;
     const float *g, *x;
@@ -157,7 +157,7 @@ int launch_bwd(BwdArgs a, PairTotal total) {
 int logprobs_bwd(const BwdArgs& a, const PairTotal& total) {
     if (a.K <= 64) return launch_bwd<4>(a, total);
     if (a.K <= 256) return launch_bwd<16>(a, total);
-    if (a.K <= 1024) return launch_bwd<64>(a, total);
+    if (a.K <= kBwdTeams) return launch_bwd<64>(a, total);
     return launch_bwd<kBwdLong>(a, total);
 }
 
@@ -426,6 +426,8 @@ JZ_API int jzhip_preference_loss(float* loss_out, float* rewards, float* logp, f
     }
     if (rc) return rc;
     if (dlogits) return logprobs_bwd(bwd, total);
-    token_fold_kernel<double><<<1, kFoldBlock, 0, stream()>>>(loss_out, losses, pairs, 0, static_cast<double>(scale));
+    // in the order of the gradient's first workgroup
+    if (K <= kBwdTeams) token_fold_kernel<kBwdBlock><<<1, kBwdBlock, 0, stream()>>>(loss_out, losses, pairs, 0, total.scale);
+    else token_fold_kernel<kBwdLong><<<1, kBwdLong, 0, stream()>>>(loss_out, losses, pairs, 0, total.scale);
     return launch_rc();
 }

@@ -553,11 +553,10 @@ __device__ __forceinline__ void fold_parts(float* out, const T* p, int n, double
     if (team.rank == 0) *out = static_cast<float>(scale * a0);
 }
 constexpr int kFoldBlock = 1024;
-template <class T>
-__global__ __launch_bounds__(kFoldBlock) void token_fold_kernel(float* out, const T* part, int n, size_t stride,
-                                                                double scale) {
-    __shared__ double slots[kFoldBlock / kWave];
-    fold_parts<kFoldBlock>(out + blockIdx.x, part + blockIdx.x * stride, n, scale, slots);
+template <int BLOCK, class T>
+__global__ __launch_bounds__(BLOCK) void token_fold_kernel(float* out, const T* part, int n, size_t stride, double scale) {
+    __shared__ double slots[BLOCK / kWave];
+    fold_parts<BLOCK>(out + blockIdx.x, part + blockIdx.x * stride, n, scale, slots);
 }
 
 // The sums over tokens of an entry point: out[k] = sum of part[k*N ...], k < count.
@@ -762,9 +761,10 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, Tok
 // 256 MB memory-side cache.
 constexpr size_t kReadTwiceBytes = size_t(96) << 20;
 
-inline int launch_token_fold(const TokenSums& sums, int N) {
+template <int BLOCK>
+int launch_token_fold(const TokenSums& sums, int N) {
     if (sums.count == 0) return 0;
-    token_fold_kernel<float><<<sums.count, kFoldBlock, 0, stream()>>>(sums.out, sums.part, N, static_cast<size_t>(N), 1.0);
+    token_fold_kernel<BLOCK, float><<<sums.count, BLOCK, 0, stream()>>>(sums.out, sums.part, N, static_cast<size_t>(N), 1.0);
     return launch_rc();
 }
 
@@ -794,7 +794,7 @@ int launch_token_chunks(Head head, const TokenSums& sums, float* scratch, float*
         const int rc = launch_rc();
         if (rc) return rc;
     }
-    return d ? 0 : launch_token_fold(sums, N);
+    return d ? 0 : launch_token_fold<kChunkBlock>(sums, N);   // in the order of the apply kernel's
 }
 
 template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
@@ -814,7 +814,7 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
     }
     kernel<<<(static_cast<unsigned>(N) + kTeams - 1) / kTeams, BLOCK, lds, stream()>>>(head, sums, d, x, K, N, ld, ldd);
     const int rc = launch_rc();
-    return rc || FOLD ? rc : launch_token_fold(sums, N);
+    return rc || FOLD ? rc : launch_token_fold<kFoldBlock>(sums, N);
 }
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
