@@ -37,6 +37,7 @@ struct Entries {
 template <bool REST>
 struct DistillHead {
     static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true, kExact = false;
+    static constexpr int kSums = 1;
     struct Early {
         float w;
         // from the prologue: REST: maximum and sum of the student's entries; sum of the q_j
@@ -47,7 +48,8 @@ struct DistillHead {
     const float* teacher;
     const int32_t* ids;
     const float *lse, *weight;   // lse set iff REST; weight may be null
-    float *token_loss, *part;    // token_loss may be null
+    float* token_loss;           // may be null
+    TokenParts to;
     float* picked;               // gradients at the entries, for a later kernel where the column is cut into chunks
     size_t ldt;
     int top;
@@ -71,11 +73,11 @@ struct DistillHead {
     __device__ bool live(size_t col, int) const { return !(weight && weight[col] == 0.f); }
     __device__ int label(size_t) const { return -1; }
     __device__ Early early(size_t col, const float*) const { return Early{weight ? weight[col] : 1.f, -INFINITY, 0.0, 0.0}; }
-    __device__ void write(size_t col, float each, float loss) const {
-        if (token_loss) token_loss[col] = each;
-        part[col] = loss;
+    __device__ void write(size_t col, double each, double loss) const {
+        if (token_loss) token_loss[col] = static_cast<float>(each);
+        to.at(col, 0) = loss;
     }
-    __device__ void idle(size_t col) const { write(col, 0.f, 0.f); }
+    __device__ void idle(size_t col) const { write(col, 0.0, 0.0); }
     // The teacher's distribution, by one wave or less; false where it has none.  all: one bit per
     // logit, cleared, left with the entries marked (null: not kept).
     template <class T>
@@ -197,7 +199,7 @@ struct DistillHead {
             if (rest > 0.0) out = r / rest;
         }
         each *= T_ * T_;
-        if (lead.rank == 0) write(col, static_cast<float>(each), static_cast<float>(w * each));
+        if (lead.rank == 0) write(col, each, w * each);
         const Grad f{static_cast<float>(T_ * w * (Q * below * inv - out)), big, static_cast<float>(T_ * w * (Q * inv)),
                      static_cast<float>(T_ * w)};
         if (chunked)
@@ -239,14 +241,15 @@ JZ_API int jzhip_distill_topk(float* loss_out, float* token_loss, float* dlogits
     if (top <= 0 || top > kMaxTop || top > K || ldt < top) return -1;
     if (!(temperature >= 1e-3f && temperature <= 1e3f)) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd), ldq = static_cast<size_t>(ldt);
-    float* part = scratch + kScratchFixed;
-    float* picked = part + static_cast<size_t>(8) * N;
+    double* part = reinterpret_cast<double*>(scratch + kScratchFixed);
+    float* picked = scratch + kScratchFixed + static_cast<size_t>(8) * N;   // behind the 8 floats a token
     const TokenSums totals{loss_out, part, 1};
+    const TokenParts to{part, static_cast<size_t>(N)};
     if (teacher_lse)
         return launch_token_kernel(DistillHead<true>{exp_scale(temperature), teacher, ids, teacher_lse, weight,
-                                                     token_loss, part, picked, ldq, top, temperature},
+                                                     token_loss, to, picked, ldq, top, temperature},
                                    totals, scratch, dlogits, logits, K, N, ldx, ldg);
     return launch_token_kernel(DistillHead<false>{exp_scale(temperature), teacher, ids, nullptr, weight, token_loss,
-                                                  part, picked, ldq, top, temperature},
+                                                  to, picked, ldq, top, temperature},
                                totals, scratch, dlogits, logits, K, N, ldx, ldg);
 }

@@ -9,6 +9,7 @@ namespace {
 template <bool ENTROPY, bool EXACT>
 struct LogprobHead {
     static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false, kExact = EXACT;
+    static constexpr int kSums = 0;
     struct Early {
         float x;   // the label's logit
     };

@@ -538,54 +538,79 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
 }
 
 // *out = scale * sum of p[0 ... n) by a wave or a workgroup of BLOCK threads, in 64 bits in a fixed order.
-template <int BLOCK, class T>
-__device__ __forceinline__ void fold_parts(float* out, const T* p, int n, double scale, double* slots) {
+template <int BLOCK>
+__device__ __forceinline__ void fold_parts(float* out, const double* p, int n, double scale, double* slots) {
     const Team<BLOCK> team{static_cast<int>(threadIdx.x % BLOCK)};
     double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
     int i = team.rank;
     for (; i + 3 * BLOCK < n; i += 4 * BLOCK) {
-        const T x0 = p[i], x1 = p[i + BLOCK], x2 = p[i + 2 * BLOCK], x3 = p[i + 3 * BLOCK];
-        a0 += static_cast<double>(x0); a1 += static_cast<double>(x1);
-        a2 += static_cast<double>(x2); a3 += static_cast<double>(x3);
+        const double x0 = p[i], x1 = p[i + BLOCK], x2 = p[i + 2 * BLOCK], x3 = p[i + 3 * BLOCK];
+        a0 += x0; a1 += x1;
+        a2 += x2; a3 += x3;
     }
-    for (; i < n; i += BLOCK) a0 += static_cast<double>(p[i]);
+    for (; i < n; i += BLOCK) a0 += p[i];
     a0 = team.reduce((a0 + a1) + (a2 + a3), AddOp{}, slots);
     if (team.rank == 0) *out = static_cast<float>(scale * a0);
 }
 constexpr int kFoldBlock = 1024;
-template <int BLOCK, class T>
-__global__ __launch_bounds__(BLOCK) void token_fold_kernel(float* out, const T* part, int n, size_t stride, double scale) {
+template <int BLOCK>
+__global__ __launch_bounds__(BLOCK) void token_fold_kernel(float* out, const double* part, int n, size_t stride, double scale) {
     __shared__ double slots[BLOCK / kWave];
     fold_parts<BLOCK>(out + blockIdx.x, part + blockIdx.x * stride, n, scale, slots);
 }
 
-// The sums over tokens of an entry point: out[k] = sum of part[k*N ...], k < count.
+// The sums over tokens of an entry point: out[k] = sum of part[k*N ...], k < count.  Parts have 64 bits: with
+// centred advantages or weights of both signs a loss is a small difference of them.
 struct TokenSums {
     float* out;
-    const float* part;
+    double* part;
     int count;
+};
+// Where a head leaves its columns' parts: sum k of column n at part[k*stride + n - first].
+struct TokenParts {
+    double* part;
+    size_t stride, first = 0;
+    __device__ __forceinline__ double& at(size_t col, int k) const { return part[static_cast<size_t>(k) * stride + (col - first)]; }
 };
 
 //   dynamic LDS: head.team_bytes(K) per team
-//   FOLD: a single workgroup holds all columns and adds up their parts itself
+//   FOLD: a single workgroup holds all columns, and its sums are the call's
+// Where a workgroup has several columns it leaves one part per sum (16384 columns of 256: 12.3 us with a part per
+// column, as 64-bit parts are 128 KB a sum to one workgroup).
 template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
 __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, TokenSums sums, float* d, const float* x,
                                                                 int K, int N, size_t ld, size_t ldd) {
     constexpr int kTeams = BLOCK / G;
+    constexpr bool kJoin = kTeams > 1 && Head::kSums > 0;
+    static_assert(!kJoin || Head::kSums <= BLOCK / kWave, "a wave per sum");
     __shared__ ColumnShared<G> shared;
+    __shared__ double parts[kJoin ? Head::kSums * kTeams : 1];
     extern __shared__ __align__(16) char dynamic[];
     const Team<G> team{static_cast<int>(kTeams > 1 ? threadIdx.x % G : threadIdx.x)};
     const int slot = kTeams > 1 ? threadIdx.x / G : 0;
-    const size_t col = static_cast<size_t>(blockIdx.x) * kTeams + slot;
+    const size_t first = static_cast<size_t>(blockIdx.x) * kTeams, col = first + slot;
+    if constexpr (kJoin) {
+        head.to = TokenParts{parts, kTeams, first};
+        if (team.rank < Head::kSums && col >= static_cast<size_t>(N)) parts[team.rank * kTeams + slot] = 0.0;
+    } else if constexpr (Head::kSums > 0) {
+        head.to.first = 0;   // known to the compiler
+    }
     if (kTeams == 1 || col < static_cast<size_t>(N)) {   // whole teams
         token_column<Head, G, NV, NT, STREAM>(head, team, shared, dynamic + static_cast<size_t>(slot) * head.team_bytes(K),
                                               col, d ? d + col * ldd : nullptr, x + col * ld, K);
     }
-    if constexpr (FOLD) {   // a wave per sum, of what this workgroup has written
+    if constexpr (kJoin) {
         __syncthreads();
-        const int k = threadIdx.x / kWave;
-        if (k < sums.count)
-            fold_parts<kWave>(sums.out + k, sums.part + static_cast<size_t>(k) * N, N, 1.0, nullptr);
+        const int k = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+        if (k < Head::kSums) {
+            double v = 0.0;
+            for (int i = lane; i < kTeams; i += kWave) v += parts[k * kTeams + i];
+            v = Team<kWave>{lane}.lanes(v, AddOp{});
+            if (lane == 0) {
+                if constexpr (FOLD) sums.out[k] = static_cast<float>(v);
+                else sums.part[static_cast<size_t>(k) * gridDim.x + blockIdx.x] = v;
+            }
+        }
     }
 }
 
@@ -761,10 +786,11 @@ __global__ __launch_bounds__(kChunkBlock) void token_apply_kernel(Head head, Tok
 // 256 MB memory-side cache.
 constexpr size_t kReadTwiceBytes = size_t(96) << 20;
 
+// n parts to a sum
 template <int BLOCK>
-int launch_token_fold(const TokenSums& sums, int N) {
+int launch_token_fold(const TokenSums& sums, int n) {
     if (sums.count == 0) return 0;
-    token_fold_kernel<BLOCK, float><<<sums.count, BLOCK, 0, stream()>>>(sums.out, sums.part, N, static_cast<size_t>(N), 1.0);
+    token_fold_kernel<BLOCK><<<sums.count, BLOCK, 0, stream()>>>(sums.out, sums.part, n, static_cast<size_t>(n), 1.0);
     return launch_rc();
 }
 
@@ -812,9 +838,10 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
             allowed.store(lds, std::memory_order_relaxed);
         }
     }
-    kernel<<<(static_cast<unsigned>(N) + kTeams - 1) / kTeams, BLOCK, lds, stream()>>>(head, sums, d, x, K, N, ld, ldd);
+    const unsigned blocks = (static_cast<unsigned>(N) + kTeams - 1) / kTeams;
+    kernel<<<blocks, BLOCK, lds, stream()>>>(head, sums, d, x, K, N, ld, ldd);
     const int rc = launch_rc();
-    return rc || FOLD ? rc : launch_token_fold<kFoldBlock>(sums, N);
+    return rc || FOLD ? rc : launch_token_fold<kFoldBlock>(sums, static_cast<int>(blocks));
 }
 template <class Head, int G, int NV, int BLOCK, bool STREAM>
 int launch_token_columns(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
@@ -823,7 +850,7 @@ int launch_token_columns(const Head& head, const TokenSums& sums, float* d, cons
         return launch_token_columns_as<Head, G, NV, BLOCK, true, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
     return launch_token_columns_as<Head, G, NV, BLOCK, false, STREAM, false>(head, sums, d, x, K, N, ld, ldd);
 }
-// teams of one wave or less: where one workgroup holds all columns, it adds up their parts as well
+// teams of one wave or less: where one workgroup holds all columns, its sums are the call's
 // (policy loss of 64 x 256: 9.0 us in two launches, 5.6 in one)
 template <class Head, int G, int NV>
 int launch_token_teams(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,

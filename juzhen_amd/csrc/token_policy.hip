@@ -15,15 +15,16 @@ namespace {
 template <bool ENTROPY>
 struct PolicyHead {
     static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true, kExact = false;
+    static constexpr int kSums = 4;
     struct Early {
         float x, old, ref, adv, w;   // x: the label's logit
     };
     ExpScale scale;
     const int32_t* labels;
     const float *old_logp, *ref_logp, *advantage, *weight;   // ref_logp, weight may be null
-    float *logp, *part;                                      // logp may be null; part: [4][N]
+    float* logp;                                             // may be null
+    TokenParts to;
     float clip_low, clip_high, kl_coef, entropy_coef;
-    int N;
 
     __host__ __device__ size_t team_bytes(int) const { return 0; }
     __device__ bool live(size_t col, int K) const {
@@ -34,15 +35,14 @@ struct PolicyHead {
         return Early{x[labels[col]], old_logp[col], ref_logp ? ref_logp[col] : 0.f, advantage[col],
                      weight ? weight[col] : 1.f};
     }
-    __device__ void write(size_t col, float lp, float loss, float kl, float cut, float h) const {
-        const size_t n = static_cast<size_t>(N);
+    __device__ void write(size_t col, float lp, double loss, double kl, double cut, double h) const {
         if (logp) logp[col] = lp;
-        part[col] = loss;
-        part[n + col] = kl;
-        part[2 * n + col] = cut;
-        part[3 * n + col] = h;
+        to.at(col, 0) = loss;
+        to.at(col, 1) = kl;
+        to.at(col, 2) = cut;
+        to.at(col, 3) = h;
     }
-    __device__ void idle(size_t col) const { write(col, 0.f, 0.f, 0.f, 0.f, 0.f); }
+    __device__ void idle(size_t col) const { write(col, 0.f, 0.0, 0.0, 0.0, 0.0); }
     template <class T>
     __device__ Grad finish(const T& lead, char*, const Early& e, size_t col, const ColumnSums& c) const {
         const double w = static_cast<double>(e.w), adv = static_cast<double>(e.adv);
@@ -73,8 +73,7 @@ struct PolicyHead {
             a += b * (h - logs);
         }
         if (lead.rank == 0)
-            write(col, static_cast<float>(lp), static_cast<float>(w * loss), static_cast<float>(w * kl),
-                  cut ? static_cast<float>(w) : 0.f, static_cast<float>(w * h));
+            write(col, static_cast<float>(lp), w * loss, w * kl, cut ? w : 0.0, w * h);
         return Grad{static_cast<float>(a * inv), static_cast<float>(b * inv), static_cast<float>(g * w), e.x};
     }
     template <class T>
@@ -98,13 +97,14 @@ JZ_API int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* sc
         return -1;
     if (kl_coef != 0.f && !ref_logp) return -1;
     const size_t ldx = static_cast<size_t>(ld), ldg = static_cast<size_t>(ldd);
-    float* part = scratch + kScratchFixed;
+    double* part = reinterpret_cast<double*>(scratch + kScratchFixed);   // the 8 floats a token
     const TokenSums totals{sums, part, 4};
+    const TokenParts to{part, static_cast<size_t>(N)};
     if (entropy_coef != 0.f)
         return launch_token_kernel(PolicyHead<true>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight,
-                                                    logp, part, clip_low, clip_high, kl_coef, entropy_coef, N},
+                                                    logp, to, clip_low, clip_high, kl_coef, entropy_coef},
                                    totals, scratch, dlogits, logits, K, N, ldx, ldg);
     return launch_token_kernel(PolicyHead<false>{exp_scale(1.0), labels, old_logp, ref_logp, advantage, weight, logp,
-                                                 part, clip_low, clip_high, kl_coef, 0.f, N},
+                                                 to, clip_low, clip_high, kl_coef, 0.f},
                                totals, scratch, dlogits, logits, K, N, ldx, ldg);
 }
