@@ -495,7 +495,8 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         f = sh.grad;
     }
     float* const to = out + span.skew;
-    const float shift = c.m == -INFINITY ? 0.f : c.m;   // (exponentials are 0 then, or NaN)
+    // No maximum: in the rest alone, whose exponentials are 0 then; else the column holds a NaN, and f.a is one.
+    const float shift = Head::kRest && c.m == -INFINITY ? 0.f : c.m;
     auto value = [&](float x) {   // (at an entry of the rest anything: its own gradient comes behind)
         const float t = x - shift;
         return grad_value<Head::kEntropy>(t, exp_shifted(t, head.scale), f.a, f.b);
