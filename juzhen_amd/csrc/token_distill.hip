@@ -36,7 +36,7 @@ struct Entries {
 
 template <bool REST>
 struct DistillHead {
-    static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true, kExact = false;
+    static constexpr bool kEntropy = false, kRest = REST, kTeacher = true, kWrites = true;
     static constexpr int kSums = 1;
     struct Early {
         float w;

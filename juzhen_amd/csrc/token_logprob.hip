@@ -8,7 +8,7 @@ namespace {
 // EXACT: log p in 64 bits as well, for a loss over many tokens.
 template <bool ENTROPY, bool EXACT>
 struct LogprobHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false, kExact = EXACT;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = false;
     static constexpr int kSums = 0;
     struct Early {
         float x;   // the label's logit
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kSmallBlock, 4) void preference_small_kernel(Logpro
         const Group g = take_group<Head>(v[r], head.scale, [](int) { return 0u; });
         group[r] = g.m;
         add_group<Head>(c[r], g, head.scale);
-        if (team.rank < span[r].odd) add_group<Head>(c[r], take_one<Head>(last[r]), head.scale);
+        if (team.rank < span[r].odd) add_group<Head>(c[r], take_one(last[r]), head.scale);
         scale_sums<Head>(c[r], team.reduce(c[r].m, LargerOp{}, static_cast<float*>(nullptr)), head.scale);
         c[r].s = team.reduce(c[r].s, AddOp{}, static_cast<double*>(nullptr));
         live[r] = live[r] && !(c[r].m == -INFINITY && c[r].s == c[r].s);

@@ -10,12 +10,12 @@
 // What bounds all of them is memory: 8 bytes per logit against about a dozen vector
 // instructions.
 //
-// Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.
-// Where a loss over many tokens cancels (the reward of an answer is a sum of small differences
-// of log-probabilities, and an error of a few 1e-8 per token shows in it), those that are 1
-// are counted apart: where one logit stands out, what the others add to its 1 is what log s
-// is made of, and fp32 rounds it at 2^-24 (Head::kExact; reading alone 61 -> 65 us for 400 MB).  What happens once per column (log s,
-// ratios, divergences) is done in 64 bits too.
+// Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.  Those
+// that are 1 are counted apart: where one logit stands out, what the others add to its 1 is what
+// log s is made of, and fp32 would round it at 2^-24, a few 1e-8 per token that show in the
+// log-probability of a likely token and in sums of small differences of them (reading alone of
+// 512 MB less a quarter 61 -> 63 us, 5000 logits a column 52 -> 54.5; beside a gradient under 1 %).
+// What happens once per column (log s, ratios, divergences) is done in 64 bits too.
 #pragma once
 
 #include "common.hpp"
@@ -246,31 +246,41 @@ __device__ __forceinline__ void store_quad(float* p, const Quad& v) {
     if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<Quad*>(p));
     else *reinterpret_cast<Quad*>(p) = v;
 }
-__device__ __forceinline__ float quad_max(const Quad& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+// The largest number of three.  (fmaxf first quiets each operand that comes from memory, an instruction per
+// logit: reading alone at 8000 logits a column 65 us with it, 63.5 without.)
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max_of(const Quad& a, const Quad& b, const Quad& c, const Quad& d) {
+    const float l = max_of(max_of(a.x, a.y, a.z), max_of(a.w, b.x, b.y), max_of(b.z, b.w, c.x));
+    const float r = max_of(max_of(c.y, c.z, c.w), max_of(d.x, d.y, d.z), d.w);
+    return max_of(l, r, r);
+}
 
 // Sums of a group of quads relative to the group's own maximum.  A thread forms them while
 // the quads behind are still on their way: exponentials need no maximum of the whole column,
 // only a factor exp(m_group - m) once that is known.
 constexpr int kGroupQuads = 4;
 struct Group {
-    float m, s, ones, et;   // exact heads: s of the exponentials below 1, ones: how many are 1
+    float m, s, ones, et;   // s: of the exponentials below 1; ones: how many are 1
 };
 // x: the group's logits; without the entropy they become e_i relative to the group.  known(k): the
 // teacher's entries among quad k, which do not count.
 template <class Head, class Known>
 __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpScale& scale, Known known) {
     Group g{-INFINITY, 0.f, 0.f, 0.f};
-    float top[kGroupQuads];
+    if constexpr (Head::kRest) {
 #pragma unroll
-    for (int k = 0; k < kGroupQuads; ++k) {
-        if constexpr (Head::kRest) {
+        for (int k = 0; k < kGroupQuads; ++k) {
             const unsigned b = known(k);
             x[k] = Quad{b & 1u ? -INFINITY : x[k].x, b & 2u ? -INFINITY : x[k].y, b & 4u ? -INFINITY : x[k].z,
                         b & 8u ? -INFINITY : x[k].w};
         }
-        top[k] = quad_max(x[k]);
     }
-    g.m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    static_assert(kGroupQuads == 4, "max_of");
+    g.m = max_of(x[0], x[1], x[2], x[3]);
     const float shift = g.m == -INFINITY ? 0.f : g.m;   // nothing but -inf: sums of 0; a NaN still shows
     float s[kGroupQuads], all[kGroupQuads], et[kGroupQuads];
 #pragma unroll
@@ -279,20 +289,15 @@ __device__ __forceinline__ Group take_group(Quad (&x)[kGroupQuads], const ExpSca
         const float e0 = exp_shifted(t0, scale), e1 = exp_shifted(t1, scale);
         const float e2 = exp_shifted(t2, scale), e3 = exp_shifted(t3, scale);
         all[k] = (e0 + e1) + (e2 + e3);
-        if constexpr (Head::kExact)   // (an exponential below 1 is its own fraction)
-            s[k] = (__builtin_amdgcn_fractf(e0) + __builtin_amdgcn_fractf(e1)) +
-                   (__builtin_amdgcn_fractf(e2) + __builtin_amdgcn_fractf(e3));
+        s[k] = (__builtin_amdgcn_fractf(e0) + __builtin_amdgcn_fractf(e1)) +   // (below 1: its own fraction)
+               (__builtin_amdgcn_fractf(e2) + __builtin_amdgcn_fractf(e3));
         if constexpr (Head::kEntropy)
-            et[k] = (e0 * fmaxf(t0, -200.f) + e1 * fmaxf(t1, -200.f)) + (e2 * fmaxf(t2, -200.f) + e3 * fmaxf(t3, -200.f));
+            et[k] = fmaf(e3, fmaxf(t3, -200.f), fmaf(e2, fmaxf(t2, -200.f), fmaf(e1, fmaxf(t1, -200.f), e0 * fmaxf(t0, -200.f))));
         else
             x[k] = Quad{e0, e1, e2, e3};
     }
-    g.s = (all[0] + all[1]) + (all[2] + all[3]);
-    if constexpr (Head::kExact) {
-        const float below = (s[0] + s[1]) + (s[2] + s[3]);
-        g.ones = rintf(g.s - below);
-        g.s = below;
-    }
+    g.s = (s[0] + s[1]) + (s[2] + s[3]);
+    g.ones = rintf(((all[0] + all[1]) + (all[2] + all[3])) - g.s);
     if constexpr (Head::kEntropy) g.et = (et[0] + et[1]) + (et[2] + et[3]);
     return g;
 }
@@ -309,7 +314,7 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
 }
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
-    ColumnSums more{g.m, (Head::kExact ? static_cast<double>(g.ones) : 0.0) + static_cast<double>(g.s) * (1.0 + kExpShort),
+    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s) * (1.0 + kExpShort),
                     static_cast<double>(g.et)};
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
@@ -318,10 +323,9 @@ __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const E
     if constexpr (Head::kEntropy) c.et += more.et;
 }
 // of a single logit
-template <class Head>
 __device__ __forceinline__ Group take_one(float x) {
     const float e = x == -INFINITY ? 0.f : x - x + 1.f;   // exp of its shift from itself; a NaN or +inf shows
-    return Group{x, Head::kExact ? 0.f : e, e, 0.f};
+    return Group{x, 0.f, e, 0.f};
 }
 
 // The compiler would interleave the independent work of an unrolled loop and spill what it
@@ -452,7 +456,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         if (team.rank < span.odd) {
             if constexpr (Head::kRest)
                 if (known_one(bits, span.single(team.rank))) last = -INFINITY;
-            add_group<Head>(c, take_one<Head>(last), head.scale);
+            add_group<Head>(c, take_one(last), head.scale);
         }
         scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
         bool filled = false;   // an entry that is not masked
@@ -576,8 +580,8 @@ struct TokenParts {
 
 //   dynamic LDS: head.team_bytes(K) per team
 //   FOLD: a single workgroup holds all columns, and its sums are the call's
-// Where a workgroup has several columns it leaves one part per sum (16384 columns of 256: 12.3 us with a part per
-// column, as 64-bit parts are 128 KB a sum to one workgroup).
+// Where a workgroup has several columns it leaves one part per sum (policy loss of 16384 columns of 256: 11.2 us, with
+// a part per column 12.3, as 64-bit parts are 128 KB a sum to one workgroup; of 1000 24.1 and 26.3).
 template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
 __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, TokenSums sums, float* d, const float* x,
                                                                 int K, int N, size_t ld, size_t ldd) {
@@ -588,7 +592,8 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
     __shared__ double parts[kJoin ? Head::kSums * kTeams : 1];
     extern __shared__ __align__(16) char dynamic[];
     const Team<G> team{static_cast<int>(kTeams > 1 ? threadIdx.x % G : threadIdx.x)};
-    const int slot = kTeams > 1 ? threadIdx.x / G : 0;
+    int slot = kTeams > 1 ? threadIdx.x / G : 0;
+    if constexpr (kTeams > 1 && G == kWave) slot = __builtin_amdgcn_readfirstlane(slot);   // a wave's column: scalar addresses
     const size_t first = static_cast<size_t>(blockIdx.x) * kTeams, col = first + slot;
     if constexpr (kJoin) {
         head.to = TokenParts{parts, kTeams, first};
@@ -675,7 +680,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_chunk_kernel(Head head, Chu
     if (team.rank < span.odd) {
         if constexpr (Head::kRest)
             if (known_one(bits, span.single(team.rank))) last = -INFINITY;
-        add_group<Head>(c, take_one<Head>(last), head.scale);
+        add_group<Head>(c, take_one(last), head.scale);
     }
     scale_sums<Head>(c, team.reduce(c.m, LargerOp{}, sh.max), head.scale);
     if constexpr (Head::kEntropy) c.et = team.reduce(c.et, AddOp{}, sh.other);

@@ -14,7 +14,7 @@ namespace {
 
 template <bool ENTROPY>
 struct PolicyHead {
-    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true, kExact = false;
+    static constexpr bool kEntropy = ENTROPY, kRest = false, kTeacher = false, kWrites = true;
     static constexpr int kSums = 4;
     struct Early {
         float x, old, ref, adv, w;   // x: the label's logit
