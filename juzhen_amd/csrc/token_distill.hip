@@ -25,12 +25,12 @@ constexpr int kMaxTop = 512;
 
 // A column's entries in LDS.
 struct Entries {
-    double* lq;   // the teacher's logit, then log q_j
-    float *q, *x;   // q_j, the student's logit
-    int* id;      // -1: none
-    static constexpr size_t kBytes = sizeof(double) + 2 * sizeof(float) + sizeof(int);
+    double *lq, *q;   // the teacher's logit, then log q_j; q_j (64 bits: the divergence is a small difference)
+    float* x;         // the student's logit
+    int* id;          // -1: none
+    static constexpr size_t kBytes = 2 * sizeof(double) + sizeof(float) + sizeof(int);
     __device__ Entries(char* own, int top)
-        : lq(reinterpret_cast<double*>(own)), q(reinterpret_cast<float*>(lq + top)), x(q + top),
+        : lq(reinterpret_cast<double*>(own)), q(lq + top), x(reinterpret_cast<float*>(q + top)),
           id(reinterpret_cast<int*>(x + top)) {}
 };
 
@@ -130,7 +130,7 @@ struct DistillHead {
                 early.s += exp64((static_cast<double>(e.x[j]) - shift) * over);
                 const double u = e.lq[j] * over - norm, q = exp64(u);
                 e.lq[j] = u;
-                e.q[j] = static_cast<float>(q);
+                e.q[j] = q;
                 Q += q;
                 some = 1.f;
             }
@@ -143,7 +143,7 @@ struct DistillHead {
                 if (e.id[j] < 0) continue;
                 const double t = e.lq[j], u = (t - static_cast<double>(big)) * over, q = exp64(u);
                 e.lq[j] = u;
-                e.q[j] = static_cast<float>(q);
+                e.q[j] = q;
                 z += q;
                 if (big != -INFINITY || t != t) some = 1.f;
             }
@@ -152,7 +152,7 @@ struct DistillHead {
             for (int j = lead.rank; j < top; j += T::kSize) {
                 if (e.id[j] < 0) continue;
                 e.lq[j] -= logz;
-                e.q[j] = static_cast<float>(static_cast<double>(e.q[j]) * inv);
+                e.q[j] *= inv;
             }
             Q = z * inv;   // 1, or NaN
         }
@@ -161,7 +161,7 @@ struct DistillHead {
     }
     // f.g: Q*T*w/s, f.x: T*w, f.b: the maximum of the whole column
     __device__ float entry_gradient(const Entries& e, int j, const Grad& f) const {
-        return exp_shifted(e.x[j] - f.b, scale) * f.g - f.x * e.q[j];
+        return static_cast<float>(static_cast<double>(exp_shifted(e.x[j] - f.b, scale) * f.g) - static_cast<double>(f.x) * e.q[j]);
     }
     template <class T>
     __device__ Grad finish(const T& lead, char* own, const Early& early, size_t col, const ColumnSums& c) const {
@@ -181,8 +181,8 @@ struct DistillHead {
         double Q = early.Q, each = 0.0;
         for (int j = lead.rank; j < top; j += T::kSize) {
             // an entry of no mass adds nothing, whatever the student gives it; a NaN stays one
-            if (e.id[j] < 0 || e.q[j] == 0.f) continue;
-            each += static_cast<double>(e.q[j]) *
+            if (e.id[j] < 0 || e.q[j] == 0.0) continue;
+            each += e.q[j] *
                     (e.lq[j] - ((static_cast<double>(e.x[j]) - static_cast<double>(big)) * over - logs));
         }
         each = lead.lanes(each, AddOp{});

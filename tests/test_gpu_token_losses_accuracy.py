@@ -210,3 +210,25 @@ def test_rewards_of_long_answers(gpu):
                         kept(columns(x, K)), kept(to_dev(labels)), kept(to_dev(rlp)), (C_.c_int * 3)(0, n, N), 1, K, K, K, 0, 1.0,
                         0.0, 0, 1.0)
     assert np.max(np.abs(to_host(rew) - want)) <= (12 * np.sqrt(n) + 0.1 * n) * U + U * np.abs(want).max()
+
+
+@pytest.mark.parametrize("K", [8, 32, 200, 500])
+@pytest.mark.parametrize("T", [1.0, 2.0])
+def test_divergence_of_nearly_equal_distributions(gpu, K, T):
+    """A student 1e-2 away from a teacher all of whose classes are known: the divergence, 5e-5, is what is left of
+    terms of 1e-2.  With the normaliser given every exponential is a 64-bit one: exp is off by 2e-13 (its series'
+    first dropped term), log by 5e-13, and they meet weights that sum to 1; the result is rounded once."""
+    N = 48
+    r = np.random.default_rng(K)
+    t = r.normal(0, 1.5, (N, K)).astype(F)
+    x = (t + r.normal(0, 1e-2, (N, K))).astype(F)
+    ids = np.tile(r.permutation(K).astype(np.int32), (N, 1))
+    tea = np.take_along_axis(t, ids.astype(np.int64), 1)
+    # a normaliser just below the true one: nothing is left for a class that the student has no mass for
+    lse = np.nextafter((np.log(np.exp(t.astype(np.float64) / T).sum(1))).astype(F), F(-100)) - F(1e-6)
+    token = ref.distill(x, tea, ids, lse, None, T)[1]
+    assert np.all(np.abs(token) < 1e-2 * T * T)
+    tok = dev_empty(N)
+    gpu.distill_topk(kept(dev_empty(1)), dptr(tok), None, kept(scratch(N, K)), kept(columns(x, K)), kept(to_dev(tea.reshape(-1))),
+                     kept(to_dev(ids.reshape(-1))), kept(to_dev(lse)), None, K, K, N, K, K, K, T)
+    same(to_host(tok), token, 2e-12 * T * T + U * np.abs(token), "token loss")
