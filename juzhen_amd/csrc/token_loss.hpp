@@ -20,8 +20,8 @@
 
 #include "common.hpp"
 
-#include <atomic>
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 namespace jz {
@@ -829,6 +829,8 @@ int launch_token_chunks(Head head, const TokenSums& sums, float* scratch, float*
     return d ? 0 : launch_token_fold<kChunkBlock>(sums, N);   // in the order of the apply kernel's
 }
 
+constexpr size_t kMaxLds = size_t(150) << 10;   // of 160 KB, beside what the kernels declare themselves
+
 template <class Head, int G, int NV, int BLOCK, bool NT, bool STREAM, bool FOLD>
 int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, const float* x, int K, int N, size_t ld,
                             size_t ldd) {
@@ -836,13 +838,13 @@ int launch_token_columns_as(const Head& head, const TokenSums& sums, float* d, c
     const size_t lds = static_cast<size_t>(kTeams) * head.team_bytes(K);
     auto kernel = token_column_kernel<Head, G, NV, BLOCK, NT, STREAM, FOLD>;
     if (lds > (size_t(64) << 10)) {   // beyond the default limit
-        static std::atomic<size_t> allowed{0};
-        if (allowed.load(std::memory_order_relaxed) < lds) {
-            const int rc = rc_of(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-            if (rc) return rc;
-            allowed.store(lds, std::memory_order_relaxed);
-        }
+        static std::once_flag once;   // per instantiation
+        static int configure_rc = 0;
+        std::call_once(once, [&] {
+            configure_rc = rc_of(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxLds)));
+        });
+        if (configure_rc) return configure_rc;
     }
     const unsigned blocks = (static_cast<unsigned>(N) + kTeams - 1) / kTeams;
     kernel<<<blocks, BLOCK, lds, stream()>>>(head, sums, d, x, K, N, ld, ldd);
@@ -871,7 +873,6 @@ int launch_token_teams(const Head& head, const TokenSums& sums, float* d, const 
 // Which way a call goes.  us on MI355X, 512 MB of logits (a quarter of the tokens unscored) unless said
 // otherwise; "values": logprobs, "gradient": the policy loss.
 constexpr int kMaxTeam = 4096, kMaxResident = 32768;
-constexpr size_t kMaxLds = size_t(150) << 10;   // of 160 KB, beside what the kernels declare themselves
 inline bool token_in_chunks(int K, int N, bool gradient) {
     // A few long columns occupy as many CUs: 1 x 262144 values 25 -> 7, gradient 41 -> 14; 64 x 131072
     // 15 -> 8.5 and 25 -> 19.  With more columns the second read of the gradient decides: 128 x 262144 gradient

@@ -133,3 +133,51 @@ def test_rest_masked_or_alone(gpu, K, N):
     same(each[3], want, (2 * (2 * np.log(K) + 8) + 4 * abs(want)) * U, "uniform")
     same(got[3][rest[3]], np.full(K - TOP, 1.0 / K - r[3] / (K - TOP)), (1.0 / K + r[3] / (K - TOP)) * (20 + 2 * np.log(K)) * U, "uniform")
     same(got[3][ids[3]], 1.0 / K - q[3], 32 * U, "uniform")
+
+
+def test_shared_memory_of_any_size_in_any_order(gpu):
+    """A bit per logit: 88, 138 and 75 KB of LDS one after another, and from two threads at once, give what each
+    gives alone."""
+    import threading
+    N, T = 70, 1.0
+    calls = {}
+    for K in (700001, 1100003, 600001):
+        r = np.random.default_rng(K)
+        x = np.zeros((N, K), F)
+        x[:, :1000] = r.normal(0, 2, (N, 1000))
+        ids = np.tile(np.array([1, 5, 999, K - 1], np.int32), (N, 1))
+        t = r.normal(0, 1, (N, TOP)).astype(F)
+        lse = np.array([lse64(v.astype(np.float64)) + 0.3 for v in t]).astype(F)
+        calls[K] = [columns(x, K), to_dev(t.reshape(-1)), to_dev(ids.reshape(-1)), to_dev(lse), scratch(N, TOP), dev_empty(1), dev_empty(N)]
+        some = [0, N - 1]
+        calls[K].append(distill64(x[some], t[some], ids[some], lse[some], np.ones(N), T)[0])
+    import torch
+    torch.cuda.synchronize()
+
+    def run(K):
+        x, t, ids, lse, sc, out, tok, _ = calls[K]
+        gpu.distill_topk(dptr(out), dptr(tok), None, dptr(sc), dptr(x), dptr(t), dptr(ids), dptr(lse), None, K, TOP, N, K, K, TOP, T)
+
+    first = {}
+    for K in (700001, 1100003, 600001, 1100003, 700001):
+        run(K)
+        got = to_host(calls[K][6])
+        same(got[[0, N - 1]], calls[K][7], (2 * (2 * np.log(K) + 8) + 2 * np.abs(calls[K][7])) * U, "token loss")
+        assert np.array_equal(first.setdefault(K, got), got)
+    failed = []
+
+    def guarded(K):
+        try:
+            run(K)
+        except Exception as e:      # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=guarded, args=(K,)) for K in (700001, 1100003)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for K in (700001, 1100003):
+        assert np.array_equal(first[K], to_host(calls[K][6]))
