@@ -441,14 +441,18 @@ int jzhip_softmax_xent_dense(float* loss_out, float* dlogits, const float* logit
  *     outputs and its gradient are 0, and its logits, log-probabilities and advantage
  *     (NaN and infinities included) are not looked at.  Entries of -inf, or of the type's
  *     lowest value beside larger ones, have probability 0 and gradient 0.  A NaN in a column
- *     that is scored reaches that column's outputs.
+ *     that is scored reaches that column's outputs.  Where a label's own probability is 0, its
+ *     log-probability is -inf and its gradient the formula's; a dL/dlogp that is infinite there
+ *     (KL term, squared preference loss) makes the column's gradient infinite or NaN, masked
+ *     entries included.
  *   - dlogits (K x N, leading dimension ldd) may be NULL where only values are wanted, and
  *     may be logits itself with ldd == ld; otherwise outputs overlap no input.  ldd - K
  *     entries behind each column are left as they are.
- *   - sixteen exponentials are added in fp32, everything further in 64 bits, as are a token's
- *     quantities (log-probability, ratio, divergence) and the sums over tokens, all in a fixed
- *     order: the same call on the same buffers gives the same bits, and values are the same
- *     with dlogits as without.  (Another address modulo 16 bytes groups a column differently.)
+ *   - sixteen exponentials are added in fp32 (those that are 1 counted apart), everything
+ *     further in 64 bits, as are a token's quantities (log-probability, ratio, divergence), its
+ *     terms of a loss and the sums over tokens, all in a fixed order: the same call on the same
+ *     buffers gives the same bits, and values are the same with dlogits as without.  (Another
+ *     address modulo 16 bytes groups a column differently.)
  *   - K up to 2^28, N up to 2^25, K * N up to 2^36, ld as int allows; offsets are 64 bits wide.
  *   - scratch: caller-provided, 16-byte aligned, jzhip_token_scratch_floats(N, top) =
  *     (8 + top) * N + 2^20 floats (top: 0 but for jzhip_distill_topk; for
@@ -483,7 +487,8 @@ int jzhip_policy_loss(float* sums, float* logp, float* dlogits, float* scratch,
 /* The paired log-ratio loss of preference data.  seq_begin: 2*pairs + 1 column numbers on the
  * HOST (read during the call; a recorded graph replays them), the first 0, never decreasing:
  * sequence s is columns [seq_begin[s], seq_begin[s+1]), 2p the chosen and 2p + 1 the rejected
- * answer of pair p; a sequence may be empty.  The columns behind the last sequence are not
+ * answer of pair p; a sequence may be empty, but not all of them (a call without tokens is
+ * refused, as everywhere here).  The columns behind the last sequence are not
  * touched.  ref_logp: log-probabilities of the same tokens under the reference model
  * (jzhip_token_logprobs), NULL for none; read for scored tokens only.
  *   R_s = beta * sum (log p(label) - ref_logp) over its scored tokens, divided by their number

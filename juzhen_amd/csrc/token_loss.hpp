@@ -3,12 +3,16 @@
 //
 // For a column x with maximum m:  t_i = x_i - m,  e_i = exp(t_i/T),  s = sum e_i,
 // p_i = e_i/s.  The shift makes every exponent <= 0, so s is in [1, K] and nothing
-// overflows.  Each kernel hands a column to a team of threads that keeps it in
-// registers between the reductions, so it is read once and its gradient written once;
-// a `Head` turns (m, s, ...) into the coefficients of that gradient,
+// overflows.  Each kernel hands a column to a team of threads; a `Head` turns (m, s, ...)
+// into the coefficients of the gradient,
 //     d_i = e_i * (a + b*t_i)  (+ corrections at the label or the teacher's entries).
-// What bounds all of them is memory: 8 bytes per logit against about a dozen vector
-// instructions.
+// What a team keeps in registers between the reductions is read once: a column of up to 4096
+// logits, and up to 65536 where there are at most two columns per CU.  With more columns a team
+// keeps 4096 (K up to 8192), 8192 (to 16384), 16384 (to 28672), all (to 32768) or 32768 logits
+// (to 65536), beyond that, and for any number of columns, 65536; the rest is read a second time
+// for the gradient, its last part first, as much of it out of the caches as fits there.  Columns
+// cut into chunks are read twice in full.  What bounds all of them is memory: 8 bytes per logit,
+// up to 12 with the second read, against about a dozen vector instructions.
 //
 // Accuracy: a thread adds sixteen exponentials in fp32 and everything further in 64 bits.  Those
 // that are 1 are counted apart: where one logit stands out, what the others add to its 1 is what
@@ -75,7 +79,8 @@ __device__ __forceinline__ double log64(double v) {
     return v == 0.0 ? -INFINITY : v == INFINITY ? v : r;
 }
 // exp(v): n = rint(v/ln 2), the Taylor series of exp(v - n ln 2) up to the tenth power
-// (|r| <= 0.347: 0.347^11/11! = 2e-13).
+// (|r| <= 0.347: 0.347^11/11! = 2e-13).  The reduction is Cody and Waite's: ln 2 as its first
+// 32 bits, whose product with n is exact, and what they leave.
 __device__ __forceinline__ double exp64(double v) {
     const double n = rint(v * 1.44269504088896340736);
     const double r = fma(n, -1.90821492927058770e-10, fma(n, -0.693147180369123816490, v));
@@ -312,10 +317,12 @@ __device__ __forceinline__ void scale_sums(ColumnSums& c, float m, const ExpScal
     c.s *= f;
     c.m = m;
 }
+__device__ __forceinline__ ColumnSums sums_of(const Group& g) {
+    return ColumnSums{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s) * (1.0 + kExpShort), static_cast<double>(g.et)};
+}
 template <class Head>
 __device__ __forceinline__ void add_group(ColumnSums& c, const Group& g, const ExpScale& scale) {
-    ColumnSums more{g.m, static_cast<double>(g.ones) + static_cast<double>(g.s) * (1.0 + kExpShort),
-                    static_cast<double>(g.et)};
+    ColumnSums more = sums_of(g);
     const float m = fmaxf(c.m, g.m);
     scale_sums<Head>(c, m, scale);
     scale_sums<Head>(more, m, scale);
@@ -389,12 +396,17 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
     typename Head::Early early{};
     if (live) {
         const unsigned* bits = nullptr;
-        auto take = [&](Quad (&x)[kGroupQuads], const ColumnTile& tile, int first) {
+        auto take = [&](Quad (&x)[kGroupQuads], const ColumnTile& tile, int first, bool only) {
             const Group g = take_group<Head>(x, head.scale, [&](int k) {
                 const int q = tile.at(first + k);
                 return known_quad(bits, span.skew + 4 * (q < span.quads ? q : 0));   // (nothing counts behind the column)
             });
-            add_group<Head>(c, g, head.scale);
+            if (only) {   // the first one
+                c = sums_of(g);
+                c.m = fmaxf(g.m, -INFINITY);   // (of nothing but NaN: none)
+            } else {
+                add_group<Head>(c, g, head.scale);
+            }
             return g.m;
         };
         // The teacher's part is the first wave's and runs while the loads of the others are under
@@ -438,7 +450,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
                 marked();
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
-                    take(v[i], tile, i * kGroupQuads);
+                    take(v[i], tile, i * kGroupQuads, false);
                     in_order<NV>();
                 }
             }
@@ -449,7 +461,7 @@ __device__ __forceinline__ void token_column(const Head& head, const Team<G>& te
         marked();
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) {
-            const float m = take(v[i], mine, i * kGroupQuads);
+            const float m = take(v[i], mine, i * kGroupQuads, !STREAM && i == 0);
             if constexpr (kKeepMax) group_max[i] = m;
             in_order<NV>();
         }
@@ -593,7 +605,9 @@ __global__ __launch_bounds__(BLOCK, 4) void token_column_kernel(Head head, Token
     extern __shared__ __align__(16) char dynamic[];
     const Team<G> team{static_cast<int>(kTeams > 1 ? threadIdx.x % G : threadIdx.x)};
     int slot = kTeams > 1 ? threadIdx.x / G : 0;
-    if constexpr (kTeams > 1 && G == kWave) slot = __builtin_amdgcn_readfirstlane(slot);   // a wave's column: scalar addresses
+    // A wave's column: scalar addresses, where registers are short (policy loss of 8192 columns of 4000 43.4 -> 40.0 us,
+    // distillation of 2000 27.6 -> 25.9; of 1000, where scalar loads wait for each other, 31.5 -> 32.7).
+    if constexpr (kTeams > 1 && G == kWave && NV > kGroupQuads) slot = __builtin_amdgcn_readfirstlane(slot);
     const size_t first = static_cast<size_t>(blockIdx.x) * kTeams, col = first + slot;
     if constexpr (kJoin) {
         head.to = TokenParts{parts, kTeams, first};
